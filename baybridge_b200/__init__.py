@@ -4,7 +4,8 @@
 ``import baybridge as cute`` surface that the hot path uses (upstream
 ``__init__.py:1-170``): ``@kernel`` / ``@jit``, ``TensorSpec``, runtime tensors,
 ``from_dlpack``, the scalar and tensor-SSA DSL, ``gemm`` / ``rmsnorm`` /
-``attention`` and ``compile(..., backend="b200")`` whose artifact launches
+``attention``, the training ops (``embedding``, ``layernorm_forward``, their
+gradients, ``adamw``) and ``compile(..., backend="b200")`` whose artifact launches
 hand-written sm_100a kernels.  ``B200Backend`` also plugs into an unmodified
 upstream checkout: ``baybridge.compile(k, ..., backend=B200Backend(),
 target=baybridge.NvidiaTarget("sm_100a"))`` or, after
@@ -41,18 +42,20 @@ from .host_values import (
     RuntimeTensor,
     Shape,
     Tensor,
+    TensorGroup,
     TensorHandle,
     clone,
     from_dlpack,
     tensor,
+    tensor_group,
     zeros,
 )
 from .trace import ReductionOp, ScalarValue, TensorValue
 from .dsl import (
     KernelDefinition,
     KernelLaunch,
-    acos, arch, asin, empty_like, full, full_like, ones_like, zeros_like, atan, atan2, attention, block_dim, block_idx, ceil, copy, cos, dim, erf, exp, exp2, floor,
-    gemm, grid_dim, jit, kernel, lane_id, layernorm, load, log, log10, log2, make_copy_atom, make_tensor, math, maximum, minimum, mma,
+    acos, adamw, arch, asin, embedding, embedding_backward, empty_like, full, full_like, ones_like, zeros_like, atan, atan2, attention, block_dim, block_idx, ceil, copy, cos, dim, erf, exp, exp2, floor,
+    gemm, grid_dim, jit, kernel, lane_id, layernorm, layernorm_backward, layernorm_forward, load, log, log10, log2, make_copy_atom, make_tensor, math, maximum, minimum, mma,
     partition, partition_program, partition_thread, barrier, program_id, rmsnorm, round, rsqrt, sin, sqrt, store, thread_idx, trunc, where,
 )
 from . import nvgpu

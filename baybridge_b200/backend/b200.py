@@ -27,14 +27,14 @@ from typing import Any, Callable
 import numpy as np
 
 from ..errors import BackendNotImplementedError
-from ..host_values import DLPACK_CUDA, RuntimeScalar, RuntimeTensor, TensorHandle, from_dlpack
+from ..host_values import DLPACK_CUDA, RuntimeScalar, RuntimeTensor, TensorGroup, TensorHandle, from_dlpack, group_signature
 from ..portable_ir import row_major_stride
 from ..scalar_types import DEVICE_NUMPY, byte_width, normalize_dtype_name
 from . import native
 from .elementwise import THREADS, UNROLL, compile_cubin, debug_bounds_enabled, render
 from . import reduction as reduction_lowering
-from .matcher import (AttentionPlan, ElementwisePlan, GemmPlan, LayerNormPlan, ReductionBundlePlan, ReductionPlan, RmsNormPlan,
-                      adopt, match)
+from .matcher import (AdamWPlan, AttentionPlan, ElementwisePlan, EmbeddingBackwardPlan, EmbeddingPlan, GemmPlan, LayerNormBackwardPlan,
+                      LayerNormForwardPlan, LayerNormPlan, ReductionBundlePlan, ReductionPlan, RmsNormPlan, adopt, match)
 
 _thread_state = threading.local()
 
@@ -120,8 +120,7 @@ class B200Backend:
             record.update(entry="bb200_reduce_bundle", parts=[self._reduction_record(part, ir) for part in plan.parts])
         else:
             record.update(asdict(plan))
-            record["entry"] = {"gemm": "bb200_gemm_bf16", "rmsnorm": "bb200_rmsnorm", "layernorm": "bb200_layernorm",
-                               "attention": "bb200_attention_fwd"}[plan.kind]
+            record["entry"] = {"gemm": "bb200_gemm_bf16", "attention": "bb200_attention_fwd"}.get(plan.kind, f"bb200_{plan.kind}")
         text = json.dumps(record, indent=1, sort_keys=True) + "\n"
         return _lowered_module_type()(backend_name=self.name, entry_point=record["entry"], dialect="b200.plan", text=text)
 
@@ -148,15 +147,18 @@ class B200Backend:
             "elementwise": self._elementwise_runner, "reduction": self._reduction_runner,
             "reduction_bundle": self._reduction_bundle_runner, "gemm": self._gemm_runner,
             "rmsnorm": self._rmsnorm_runner, "layernorm": self._layernorm_runner, "attention": self._attention_runner,
+            "embedding": self._embedding_runner, "embedding_backward": self._embedding_backward_runner,
+            "layernorm_forward": self._layernorm_forward_runner, "layernorm_backward": self._layernorm_backward_runner,
+            "adamw": self._adamw_runner,
         }[plan.kind](ir, plan, record, state)
         arguments = ir.arguments
         # what a device tensor handle must look like per argument, computed once
         expected = [(tuple(a.spec.shape), a.spec.dtype, row_major_stride(a.spec.shape)) if a.kind == "tensor" else None for a in arguments]
         tensor_positions = [position for position, a in enumerate(arguments) if a.kind == "tensor"]
         all_tensors = len(tensor_positions) == len(arguments)
-        # kernels that can record a code in the device status word: the mbarrier pipelines (bounded waits) and the
-        # bounds-checking debug build of thread-by-thread elementwise kernels
-        waits_on_device = plan.kind in ("gemm", "attention") or bool(record.get("debug_bounds"))
+        # kernels that can record a code in the device status word: the mbarrier pipelines (bounded waits), the
+        # bounds-checking debug build of thread-by-thread elementwise kernels, and the lookups (tokens outside the table)
+        waits_on_device = plan.kind in ("gemm", "attention", "embedding", "embedding_backward") or bool(record.get("debug_bounds"))
         checked: dict[tuple[int, int], Any] = {}  # (argument position, id of handle) -> handle already validated there
 
         def launcher(*args: Any, **kwargs: Any) -> None:
@@ -216,6 +218,8 @@ class B200Backend:
                         # a bounded in-kernel wait that gave up leaves partial output: surface it like a native launch
                         # that returned non-zero (upstream hipcc_exec.py:181-182)
                         status = native.take_device_status(stream_handle)
+                        if status == native.TOKEN_OUT_OF_RANGE:
+                            raise RuntimeError(f"launch_{ir.name} returned device status {status}: a token lies outside the table's rows")
                         if status:
                             raise RuntimeError(f"launch_{ir.name} returned device status {status}: a bounded device-side wait "
                                                f"gave up ({native.ERROR_NAMES[-6]}); the output is incomplete")
@@ -243,6 +247,8 @@ class B200Backend:
                     native.library().bb200_module_unload(module)
                 holder.get("functions", {}).clear()
 
+        if isinstance(plan, AdamWPlan):
+            launcher.grouped = self._adamw_grouped(ir, plan, state)  # type: ignore[attr-defined]
         launcher.plan = plan  # type: ignore[attr-defined]
         launcher.release = release  # type: ignore[attr-defined]
         return launcher
@@ -529,6 +535,112 @@ class B200Backend:
                         int(plan.causal), stream_handle)
 
         return run
+
+    def _embedding_runner(self, ir, plan: EmbeddingPlan, record, state):
+        entry, codes = native.entry_point("bb200_embedding"), native.DTYPE_CODES
+        dtypes = codes[plan.table_dtype], codes[plan.out_dtype], codes[plan.token_dtype]
+
+        def run(pointers, scalars, stream_handle) -> None:
+            native.call_resolved(entry, "bb200_embedding", *dtypes, pointers[plan.tokens], pointers[plan.table], pointers[plan.out],
+                                 plan.count, plan.vocabulary, plan.hidden, plan.scale, stream_handle)
+
+        return run
+
+    def _embedding_backward_runner(self, ir, plan: EmbeddingBackwardPlan, record, state):
+        entry, codes = native.entry_point("bb200_embedding_backward"), native.DTYPE_CODES
+        dtypes = codes[plan.grad_dtype], codes[plan.table_dtype], codes[plan.token_dtype]
+
+        def run(pointers, scalars, stream_handle) -> None:
+            native.call_resolved(entry, "bb200_embedding_backward", *dtypes, pointers[plan.grad_out], pointers[plan.tokens],
+                                 pointers[plan.grad_table], plan.count, plan.vocabulary, plan.hidden, plan.scale, plan.padding_token,
+                                 int(plan.accumulate), stream_handle)
+
+        return run
+
+    def _layernorm_forward_runner(self, ir, plan: LayerNormForwardPlan, record, state):
+        entry, codes = native.entry_point("bb200_layernorm_forward"), native.DTYPE_CODES
+        dtypes = codes[plan.dtype], codes[plan.weight_dtype]
+        order = (plan.x, plan.residual, plan.weight, plan.bias, plan.out, plan.out_resid, plan.mean, plan.rstd)
+
+        def run(pointers, scalars, stream_handle) -> None:
+            native.call_resolved(entry, "bb200_layernorm_forward", *dtypes,
+                                 *[None if position is None else pointers[position] for position in order],
+                                 plan.rows, plan.hidden, plan.epsilon, stream_handle)
+
+        return run
+
+    def _layernorm_backward_runner(self, ir, plan: LayerNormBackwardPlan, record, state):
+        entry, codes = native.entry_point("bb200_layernorm_backward"), native.DTYPE_CODES
+        dtypes = codes[plan.dtype], codes[plan.weight_dtype]
+        order = (plan.grad_out, plan.x, plan.mean, plan.rstd, plan.weight, plan.grad_resid, plan.grad_x, plan.grad_weight, plan.grad_bias)
+
+        def run(pointers, scalars, stream_handle) -> None:
+            native.call_resolved(entry, "bb200_layernorm_backward", *dtypes,
+                                 *[None if position is None else pointers[position] for position in order],
+                                 plan.rows, plan.hidden, stream_handle)
+
+        return run
+
+    @staticmethod
+    def _adamw_call(plan: AdamWPlan):
+        """``step(lists, schedule, stream)``: ``lists`` are the address arrays of params, grads, exp_avgs, exp_avg_sqs, masters."""
+        entry, count = native.entry_point("bb200_adamw"), len(plan.params)
+        numels = (ctypes.c_size_t * count)(*plan.numels)
+        param_dtypes = (ctypes.c_int * count)(*(native.DTYPE_CODES[name] for name in plan.param_dtypes))
+        grad_dtypes = (ctypes.c_int * count)(*(native.DTYPE_CODES[name] for name in plan.grad_dtypes))
+        decays = (ctypes.c_float * count)(*plan.weight_decay)
+
+        def step(lists, schedule, stream_handle) -> None:
+            native.call_resolved(entry, "bb200_adamw", count, numels, param_dtypes, grad_dtypes, decays, *lists, schedule,
+                                 plan.beta1, plan.beta2, plan.epsilon, stream_handle)
+
+        return step
+
+    def _adamw_runner(self, ir, plan: AdamWPlan, record, state):
+        step, count = self._adamw_call(plan), len(plan.params)
+        roles = (plan.params, plan.grads, plan.exp_avgs, plan.exp_avg_sqs, plan.masters)
+
+        def run(pointers, scalars, stream_handle) -> None:
+            lists = [(ctypes.c_void_p * count)(*[pointers[position] for position in role]) if role else None for role in roles]
+            step(lists, pointers[plan.schedule], stream_handle)
+
+        return run
+
+    def _adamw_grouped(self, ir, plan: AdamWPlan, state):
+        """The step on whole tensor groups: ``grouped({position of the first leaf: value}, stream)`` launches and returns
+        True when every list of the plan arrives as one ``TensorGroup``, and returns False otherwise (the caller then
+        passes the leaves one by one)."""
+        step, count = self._adamw_call(plan), len(plan.params)
+        roles = [plan.params, plan.grads, plan.exp_avgs, plan.exp_avg_sqs] + ([plan.masters] if plan.masters else [])
+        contiguous = all(role == tuple(range(role[0], role[0] + count)) for role in roles)
+        expected = [group_signature((ir.arguments[p].spec.dtype, ir.arguments[p].spec.shape) for p in role) for role in roles]
+        names = ("params", "grads", "exp_avgs", "exp_avg_sqs", "masters")
+
+        def grouped(values: dict[int, Any], stream: Any) -> bool:
+            schedule = values.get(plan.schedule)
+            if not contiguous or type(schedule) is not TensorHandle or len(values) != len(roles) + 1:
+                return False
+            groups = [values.get(role[0]) for role in roles]
+            if any(type(group) is not TensorGroup for group in groups):
+                return False
+            for name, group, signature in zip(names, groups, expected):
+                if group.signature != signature:
+                    raise TypeError(f"b200: the {name} of {ir.name} differ in number, dtype or shape from those it was compiled for")
+                if group.device_id != schedule.device_id:
+                    raise BackendNotImplementedError("b200: tensor arguments live on different devices")
+            if schedule.device_type != DLPACK_CUDA or schedule.shape != (3,) or schedule.dtype != "f32" or not schedule.is_contiguous:
+                raise TypeError(f"b200 tensor argument '{ir.arguments[plan.schedule].name}' expects a dense CUDA f32 tensor of shape (3,)")
+            native.require_device()
+            _bind_device(int(schedule.device_id))
+            stream_handle = native.stream_handle(stream)
+            lists = [group.addresses for group in groups]
+            step(lists if plan.masters else lists + [None], schedule.data_ptr(), stream_handle)
+            LAUNCH_COUNTER["launches"] += 1
+            if self.synchronize and not native.recording():
+                native.call("bb200_stream_synchronize", stream_handle)
+            return True
+
+        return grouped
 
 
 def install_into_upstream(module: Any = None) -> None:

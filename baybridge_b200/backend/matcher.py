@@ -2,7 +2,9 @@
 
 ``match(ir)`` classifies a traced kernel as one of
 
-* ``GemmPlan`` / ``RmsNormPlan`` / ``AttentionPlan`` — a single explicit op whose
+* ``GemmPlan`` / ``RmsNormPlan`` / ``AttentionPlan`` and the plans of the training
+  ops (``EmbeddingPlan``, ``LayerNormForwardPlan``, their backward plans,
+  ``AdamWPlan``) — a single explicit op whose
   operands are kernel arguments (the "single explicit op" rule of upstream
   ``hipkittens_ref.py:88-275`` and ``hipkittens_exec.py:631-894``), or
 * ``ElementwisePlan`` — a load / scalar-expression / store body, in the indexed
@@ -120,6 +122,94 @@ class AttentionPlan:
     causal: bool
     dtype: str
     kind: str = "attention"
+
+
+@dataclass(frozen=True)
+class EmbeddingPlan:
+    tokens: int
+    table: int
+    out: int
+    count: int
+    vocabulary: int
+    hidden: int
+    scale: float
+    token_dtype: str
+    table_dtype: str
+    out_dtype: str
+    kind: str = "embedding"
+
+
+@dataclass(frozen=True)
+class EmbeddingBackwardPlan:
+    grad_out: int
+    tokens: int
+    grad_table: int
+    count: int
+    vocabulary: int
+    hidden: int
+    scale: float
+    padding_token: int  # -1 = none
+    accumulate: bool
+    token_dtype: str
+    grad_dtype: str
+    table_dtype: str
+    kind: str = "embedding_backward"
+
+
+@dataclass(frozen=True)
+class LayerNormForwardPlan:
+    x: int
+    residual: int | None
+    weight: int
+    bias: int | None
+    out: int
+    out_resid: int | None
+    mean: int
+    rstd: int
+    rows: int
+    hidden: int
+    epsilon: float
+    dtype: str
+    weight_dtype: str
+    kind: str = "layernorm_forward"
+
+
+@dataclass(frozen=True)
+class LayerNormBackwardPlan:
+    grad_out: int
+    x: int
+    mean: int
+    rstd: int
+    weight: int
+    grad_resid: int | None
+    grad_x: int
+    grad_weight: int
+    grad_bias: int | None
+    rows: int
+    hidden: int
+    dtype: str
+    weight_dtype: str
+    kind: str = "layernorm_backward"
+
+
+@dataclass(frozen=True)
+class AdamWPlan:
+    """The i-th tensors of ``params``, ``grads``, ``exp_avgs``, ``exp_avg_sqs`` and ``masters`` (empty = none) belong together."""
+
+    params: tuple[int, ...]
+    grads: tuple[int, ...]
+    exp_avgs: tuple[int, ...]
+    exp_avg_sqs: tuple[int, ...]
+    masters: tuple[int, ...]
+    schedule: int
+    numels: tuple[int, ...]
+    param_dtypes: tuple[str, ...]
+    grad_dtypes: tuple[str, ...]
+    weight_decay: tuple[float, ...]
+    beta1: float
+    beta2: float
+    epsilon: float
+    kind: str = "adamw"
 
 
 @dataclass(frozen=True)
@@ -371,6 +461,103 @@ def _match_attention(ir, op) -> AttentionPlan:
     if head_dim not in (64, 128) and seq > 8192:
         raise _unsupported(f"attention with head_dim {head_dim} (not 64/128) is limited to seq <= 8192 (got {seq})")
     return AttentionPlan(q, k, v, out, lse, batch, seq, heads, kv_heads, head_dim, bool(op.attrs.get("causal")), "bf16")
+
+
+def _embedding_shapes(ir, tokens_spec, table_spec, rows_spec, what: str) -> tuple[int, int, int]:
+    if tokens_spec.dtype not in ("i32", "i64"):
+        raise _unsupported(f"{what} tokens must be i32 or i64 (got {tokens_spec.dtype})")
+    if len(table_spec.shape) != 2 or tuple(rows_spec.shape) != tuple(tokens_spec.shape) + (table_spec.shape[1],):
+        raise _unsupported(f"{what} requires a rank-2 table and rows of shape tokens + (hidden,)")
+    if table_spec.dtype not in FLOAT_DTYPES or rows_spec.dtype not in FLOAT_DTYPES:
+        raise _unsupported(f"{what} requires f32/bf16/f16 tensors (got {table_spec.dtype}, {rows_spec.dtype})")
+    vocabulary, hidden = table_spec.shape
+    for extent in (tokens_spec.numel, vocabulary, hidden):
+        if extent >= 2**31 - 1:
+            raise _unsupported(f"{what} extents must be below 2^31 - 1 (got {extent})")
+    return tokens_spec.numel, vocabulary, hidden
+
+
+def _match_embedding(ir, op) -> EmbeddingPlan:
+    positions = _argument_positions(ir)
+    (tokens, ts), (table, vs), (out, os_) = (_tensor_arg(ir, positions, name, "embedding") for name in op.inputs)
+    count, vocabulary, hidden = _embedding_shapes(ir, ts, vs, os_, "embedding")
+    return EmbeddingPlan(tokens, table, out, count, vocabulary, hidden, float(op.attrs["scale"]), ts.dtype, vs.dtype, os_.dtype)
+
+
+def _match_embedding_backward(ir, op) -> EmbeddingBackwardPlan:
+    positions = _argument_positions(ir)
+    (grad_out, gs), (tokens, ts), (grad_table, vs) = (_tensor_arg(ir, positions, name, "embedding_backward") for name in op.inputs)
+    count, vocabulary, hidden = _embedding_shapes(ir, ts, vs, gs, "embedding_backward")
+    padding = op.attrs.get("padding_token")
+    return EmbeddingBackwardPlan(grad_out, tokens, grad_table, count, vocabulary, hidden, float(op.attrs["scale"]),
+                                 -1 if padding is None else int(padding), bool(op.attrs["accumulate"]), ts.dtype, gs.dtype, vs.dtype)
+
+
+def _norm_shapes(x_spec, same, vectors, stats, what: str) -> tuple[int, int]:
+    """(rows, hidden) after the checks that the training norms share."""
+    if not x_spec.shape or x_spec.dtype not in FLOAT_DTYPES:
+        raise _unsupported(f"{what} requires f32/bf16/f16 tensors of rank >= 1")
+    hidden = x_spec.shape[-1]
+    rows = x_spec.numel // hidden
+    if any(spec.shape != x_spec.shape or spec.dtype != x_spec.dtype for spec in same):
+        raise _unsupported(f"{what} requires its row tensors of one shape and dtype")
+    if any(spec.shape != (hidden,) or spec.dtype != vectors[0].dtype or spec.dtype not in (x_spec.dtype, "f32") for spec in vectors):
+        raise _unsupported(f"{what} requires weight and bias vectors [hidden] of one dtype, x's or f32")
+    if any(spec.numel != rows or spec.dtype != "f32" for spec in stats):
+        raise _unsupported(f"{what} requires f32 mean and rstd, one value per row")
+    limit = 16384 if x_spec.dtype == "f32" else 32768
+    if hidden > limit or rows >= 2**31 - 1:
+        raise _unsupported(f"{what} hidden size {hidden} must be at most {limit} for {x_spec.dtype}, and rows below 2^31 - 1")
+    return rows, hidden
+
+
+def _match_layernorm_forward(ir, op) -> LayerNormForwardPlan:
+    positions = _argument_positions(ir)
+    operands = [_tensor_arg(ir, positions, name, "layernorm_forward") for name in op.inputs]
+    (x, xs), (out, os_), (mean, ms), (rstd, rs), (weight, ws), *rest = operands
+    bias, bs = rest.pop(0) if op.attrs["bias"] else (None, None)
+    (residual, res), (out_resid, ors) = rest if op.attrs["residual"] else ((None, None), (None, None))
+    rows, hidden = _norm_shapes(xs, [s for s in (os_, res, ors) if s is not None], [s for s in (ws, bs) if s is not None], (ms, rs),
+                                "layernorm_forward")
+    return LayerNormForwardPlan(x, residual, weight, bias, out, out_resid, mean, rstd, rows, hidden, float(op.attrs["epsilon"]),
+                                xs.dtype, ws.dtype)
+
+
+def _match_layernorm_backward(ir, op) -> LayerNormBackwardPlan:
+    positions = _argument_positions(ir)
+    operands = [_tensor_arg(ir, positions, name, "layernorm_backward") for name in op.inputs]
+    (grad_out, gs), (x, xs), (mean, ms), (rstd, rs), (weight, ws), (grad_x, gxs), (grad_weight, gws), *rest = operands
+    grad_bias, gbs = rest.pop(0) if op.attrs["bias"] else (None, None)
+    grad_resid, grs = rest.pop(0) if op.attrs["residual"] else (None, None)
+    rows, hidden = _norm_shapes(xs, [s for s in (gs, gxs, grs) if s is not None], [s for s in (ws, gws, gbs) if s is not None], (ms, rs),
+                                "layernorm_backward")
+    return LayerNormBackwardPlan(grad_out, x, mean, rstd, weight, grad_resid, grad_x, grad_weight, grad_bias, rows, hidden, xs.dtype, ws.dtype)
+
+
+def _match_adamw(ir, op) -> AdamWPlan:
+    positions = _argument_positions(ir)
+    operands = [_tensor_arg(ir, positions, name, "adamw") for name in op.inputs]
+    count, with_masters = int(op.attrs["count"]), bool(op.attrs["masters"])
+    if len(operands) != count * (5 if with_masters else 4) + 1:
+        raise _unsupported(f"adamw of {count} tensors got {len(operands)} operands")
+    schedule, schedule_spec = operands.pop()
+    if schedule_spec.shape != (3,) or schedule_spec.dtype != "f32":
+        raise _unsupported("adamw schedule must be f32 (3,)")
+    if len({position for position, _ in operands}) != len(operands):
+        raise _unsupported("adamw was given the same tensor argument twice")
+    params, grads, exp_avgs, exp_avg_sqs = (operands[k * count:(k + 1) * count] for k in range(4))
+    masters = operands[4 * count:]
+    for index, (_, spec) in enumerate(params):
+        group = [grads[index][1], exp_avgs[index][1], exp_avg_sqs[index][1]] + ([masters[index][1]] if with_masters else [])
+        if any(other.shape != spec.shape for other in group) or any(other.dtype != "f32" for other in group[1:]):
+            raise _unsupported(f"adamw tensors {index} differ in shape, or their moments or masters are not f32")
+        if spec.dtype not in FLOAT_DTYPES or group[0].dtype not in (spec.dtype, "f32"):
+            raise _unsupported(f"adamw parameter {index} must be f32/bf16/f16 with a gradient of its dtype or f32")
+    place = lambda pairs: tuple(position for position, _ in pairs)  # noqa: E731
+    return AdamWPlan(place(params), place(grads), place(exp_avgs), place(exp_avg_sqs), place(masters), schedule,
+                     tuple(spec.numel for _, spec in params), tuple(spec.dtype for _, spec in params),
+                     tuple(spec.dtype for _, spec in grads), tuple(float(item) for item in op.attrs["weight_decay"]),
+                     float(op.attrs["betas"][0]), float(op.attrs["betas"][1]), float(op.attrs["epsilon"]))
 
 
 # ---------------------------------------------------------------------------------------------
@@ -1113,7 +1300,11 @@ def adopt(ir):
     return ir if isinstance(ir, PortableKernelIR) else PortableKernelIR.from_dict(ir.to_dict())
 
 
-EXPLICIT = {"mma": _match_gemm, "rmsnorm": _match_rmsnorm, "layernorm": _match_layernorm, "attention": _match_attention}
+EXPLICIT = {
+    "mma": _match_gemm, "rmsnorm": _match_rmsnorm, "layernorm": _match_layernorm, "attention": _match_attention,
+    "embedding": _match_embedding, "embedding_backward": _match_embedding_backward, "layernorm_forward": _match_layernorm_forward,
+    "layernorm_backward": _match_layernorm_backward, "adamw": _match_adamw,
+}
 
 
 def match(ir):

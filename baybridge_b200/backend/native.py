@@ -36,6 +36,7 @@ ERROR_NAMES = {
     -1: "BB200_E_INVALID_ARGUMENT", -2: "BB200_E_UNSUPPORTED_SHAPE", -3: "BB200_E_MISALIGNED",
     -4: "BB200_E_NO_DRIVER", -5: "BB200_E_NOT_SM100", -6: "BB200_E_DEVICE_TIMEOUT", -7: "BB200_E_TOO_LARGE",
 }
+TOKEN_OUT_OF_RANGE = 311  # device status word: a lookup met a token outside its table
 DTYPE_CODES = {"f32": 0, "bf16": 1, "f16": 2, "i32": 3, "i64": 4, "index": 4, "i8": 5, "i1": 6}
 BINARY_OP_CODES = {"add": 0, "sub": 1, "mul": 2, "div": 3, "max": 4, "min": 5}
 
@@ -162,6 +163,12 @@ PROTOTYPES: dict[str, list[Any]] = {
     "bb200_gemm_bf16_gather": [P, P, ctypes.POINTER(P), I, I, I, I, I, I, I, I, P],
     "bb200_attention_fwd": [P, P, P, P, P, I, I, I, I, I, I, P],
     "bb200_attention_fwd_gather": [P, P, P, ctypes.POINTER(P), ctypes.POINTER(P), I, I, I, I, I, I, I, I, P],
+    "bb200_embedding": [I, I, I, P, P, P, Z, Z, Z, ctypes.c_float, P],
+    "bb200_embedding_backward": [I, I, I, P, P, P, Z, Z, Z, ctypes.c_float, ctypes.c_int64, I, P],
+    "bb200_layernorm_forward": [I, I, P, P, P, P, P, P, P, P, Z, Z, ctypes.c_float, P],
+    "bb200_layernorm_backward": [I, I, P, P, P, P, P, P, P, P, P, Z, Z, P],
+    "bb200_adamw": [I, ctypes.POINTER(Z), ctypes.POINTER(I), ctypes.POINTER(I), ctypes.POINTER(ctypes.c_float), PP, PP, PP, PP, PP, P,
+                    ctypes.c_double, ctypes.c_double, ctypes.c_float, P],
     "bb200_take_device_status": [P, ctypes.POINTER(I)],
     "bb200_selftest_bounded_wait": [ctypes.c_uint, P],
     "bb200_device_status_address": [PP],

@@ -73,4 +73,41 @@ int encode_tensormap_3d(void* map_out, bb200_dtype dtype, const void* base, uint
                         uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0, uint32_t box1, uint32_t box2,
                         int swizzle);
 
+// ---- stream-ordered workspaces (workspace.cu) ------------------------------------------------------------------------
+// Devices that per-device tables of this library cover.
+constexpr int kMaxWorkspaceDevices = 64;
+
+// The pool that workspaces of `device` come from (nullptr: it could not be created).  A pool of this library's own that
+// keeps what is freed (release threshold = everything): the device's default pool hands memory back at every
+// synchronisation, and a caller that synchronises between two calls would then pay a fresh allocation (about 130 us)
+// for every call.
+cudaMemPool_t workspace_pool(int device);
+
+// Streaming multiprocessors of the current device.
+int multiprocessor_count();
+
+// Memory for one call: taken in stream order from the current device's pool, given back in stream order by release()
+// (or the destructor).  Two calls, on one stream or on several, never share it; recorded into a launch graph it becomes
+// an allocation of that graph's own.
+class Workspace {
+ public:
+  explicit Workspace(cudaStream_t stream) : stream_(stream) {}
+  ~Workspace() { release(nullptr); }
+  Workspace(const Workspace&) = delete;
+  Workspace& operator=(const Workspace&) = delete;
+  int take(size_t bytes, const char* what);  // a status; data() is 256-byte aligned afterwards
+  int release(const char* what);             // a status; `what` names the caller in the error text
+  char* data() const { return data_; }
+
+ private:
+  cudaStream_t stream_;
+  char* data_ = nullptr;
+};
+
+// Whether [a, a + a_bytes) and [b, b + b_bytes) share memory (null pointers share none).
+inline bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x && y && x < y + b_bytes && y < x + a_bytes;
+}
+
 }  // namespace bb200

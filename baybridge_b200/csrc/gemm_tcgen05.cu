@@ -960,31 +960,6 @@ int split_k_count(int tiles, int k_blocks, int sms) {
   return splits < 2 ? 1 : splits;
 }
 
-// Split-K workspaces come from a pool of this library's own that keeps what is freed (release threshold = everything):
-// the device's default pool hands memory back at every synchronisation, and a caller that synchronises between two GEMMs
-// would then pay a fresh allocation (≈ 130 us) for every call.
-cudaMemPool_t workspace_pool(int device) {
-  static std::mutex guard;
-  static cudaMemPool_t pools[kMaxDevices] = {};
-  std::lock_guard<std::mutex> lock(guard);
-  if (!pools[device]) {
-    cudaMemPoolProps props = {};
-    props.allocType = cudaMemAllocationTypePinned;
-    props.handleTypes = cudaMemHandleTypeNone;
-    props.location.type = cudaMemLocationTypeDevice;
-    props.location.id = device;
-    cudaMemPool_t created = nullptr;
-    if (cudaMemPoolCreate(&created, &props) != cudaSuccess) {
-      cudaGetLastError();
-      return nullptr;
-    }
-    unsigned long long keep_everything = ~0ull;
-    cudaMemPoolSetAttribute(created, cudaMemPoolAttrReleaseThreshold, &keep_everything);
-    pools[device] = created;
-  }
-  return pools[device];
-}
-
 template <typename OutT, bool A_MN, bool B_MN, int TN>
 int launch_single(const void* a_operand, const void* b, const Destinations& dst, int m, int n, int k, int device, int sms, bool may_split,
                   cudaStream_t stream) {

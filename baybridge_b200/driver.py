@@ -26,7 +26,7 @@ from pathlib import Path
 from typing import Any, Callable
 
 from .errors import BackendNotImplementedError, CompilationError
-from .host_values import TensorHandle, infer_runtime_spec, normalize_runtime_argument
+from .host_values import TensorGroup, TensorHandle, infer_runtime_spec, normalize_runtime_argument
 from .portable_ir import PortableKernelIR, ScalarSpec, TensorSpec
 from .targets import B200, AMDTarget, NvidiaTarget
 from .trace import IRBuilder, ScalarValue, TensorValue, tracing
@@ -116,7 +116,7 @@ def _proxy_for(parameter: str, value: Any, builder: IRBuilder, bindings: list[di
         spec = ScalarSpec(dtype) if shape is None else TensorSpec(shape=shape, dtype=dtype)
         suffix = "".join("_" + str(item).replace("-", "_") for item in path)
         return _bind_leaf(builder, bindings, parameter, parameter + suffix, spec, path)
-    if isinstance(value, (list, tuple)):
+    if isinstance(value, (list, tuple, TensorGroup)):
         walked = [_proxy_for(parameter, item, builder, bindings, path + (i,)) for i, item in enumerate(value)]
         return walked if isinstance(value, list) else tuple(walked)
     if isinstance(value, dict):
@@ -271,6 +271,12 @@ def _bind_user_arguments(definition, backend_launcher: Callable[..., Any], bindi
     direct = (len(positional) == len(parameters) and "stream" not in signature.parameters
               and all(not binding["path"] and binding["parameter"] in positional for binding in bindings))
     order = [positional.index(binding["parameter"]) for binding in bindings] if direct else []
+    # a backend launcher that takes whole tensor groups (one argument for a list of leaves) is offered them first:
+    # per parameter that has leaves, its place in the call and the position of its first leaf
+    flat = all(binding["parameter"] in positional and len(binding["path"]) <= 1 for binding in bindings)
+    grouped = getattr(backend_launcher, "grouped", None) if flat else None
+    spans = [(positional.index(binding["parameter"]), leaf) for leaf, binding in enumerate(bindings)
+             if grouped is not None and binding["path"] in ([], [0])]
 
     def launcher(*args: Any, **kwargs: Any) -> Any:
         if direct and len(args) == len(positional) and (not kwargs or (len(kwargs) == 1 and "stream" in kwargs)):
@@ -281,6 +287,9 @@ def _bind_user_arguments(definition, backend_launcher: Callable[..., Any], bindi
                     leaves = [normalize_runtime_argument(value, stream=stream) for value in leaves]
                     break
             return backend_launcher(*leaves) if stream is None else backend_launcher(*leaves, stream=stream)
+        if grouped is not None and len(args) == len(positional) and not kwargs.keys() - {"stream"}:
+            if grouped({leaf: args[place] for place, leaf in spans}, kwargs.get("stream")):
+                return None
         stream = None if "stream" in signature.parameters else kwargs.pop("stream", None)
         bound = signature.bind_partial(*args, **kwargs).arguments
         if stream is None and "stream" in bound:

@@ -6,7 +6,9 @@ path exercises: ``kernel``/``jit`` decorators and launch objects
 ``load``/``store`` with optional predicates (``:2931-3019``), whole-tensor
 ``copy`` (``:3357-3415``), ``where`` (``:2538-2600``), the ``math`` namespace
 (``math.py:13-76``), and the explicit ops ``gemm``/``mma`` (``frontend.py:3684-3740,
-4052-4091``), ``rmsnorm`` (``:3828-3874``) and ``attention`` (``:3877-3968``).
+4052-4091``), ``rmsnorm`` (``:3828-3874``) and ``attention`` (``:3877-3968``);
+next to them stand the ops of a training step that upstream lacks: ``embedding``,
+``layernorm_forward``, their gradients, and ``adamw``.
 
 Upstream entry points are dual-mode (emit IR while tracing, otherwise execute
 on the CPU).  Here they are trace-only; calling one with host tensors outside
@@ -671,3 +673,161 @@ def attention(q: Any, k: Any, v: Any, out: Any, lse: Any, *, causal: bool = Fals
         raise ValueError("baybridge.attention requires matching q/k/v/out dtypes")
     require_builder().emit_void("attention", q, k, v, out, lse, attrs={"causal": bool(causal)})
     return out
+
+
+# ---------------------------------------------------------------------------------------------
+# explicit ops of a training step: embedding, LayerNorm with its gradient, AdamW.  Upstream has none of them.
+# ---------------------------------------------------------------------------------------------
+_FLOATS = ("f32", "bf16", "f16")
+
+
+def _float_tensor(value: TensorValue, op: str, name: str) -> None:
+    if value.spec.dtype not in _FLOATS:
+        raise ValueError(f"baybridge.{op} expects {name} of dtype f32, bf16 or f16, got {value.spec.dtype}")
+
+
+def _embedding_operands(tokens: TensorValue, table: TensorValue, rows: TensorValue, op: str, rows_name: str) -> None:
+    if tokens.spec.dtype not in ("i32", "i64"):
+        raise ValueError(f"baybridge.{op} expects tokens of dtype i32 or i64, got {tokens.spec.dtype}")
+    if table.ndim != 2:
+        raise ValueError(f"baybridge.{op} expects a rank-2 table [vocabulary, hidden], got {table.spec.shape}")
+    if rows.spec.shape != tokens.spec.shape + (table.spec.shape[1],):
+        raise ValueError(f"baybridge.{op} expects {rows_name} shape {tokens.spec.shape + (table.spec.shape[1],)}, got {rows.spec.shape}")
+    _float_tensor(table, op, "a table")
+    _float_tensor(rows, op, rows_name)
+
+
+def embedding(tokens: Any, table: Any, out: Any, *, scale: float = 1.0) -> Any:
+    """``out[..., :] = scale * table[tokens[...], :]``, computed in 32 bits and rounded once to ``out``'s dtype.
+
+    ``tokens`` (i32 or i64) has any shape, ``table`` is ``[vocabulary, hidden]``, ``out`` is ``tokens.shape + (hidden,)``;
+    table and out are f32, bf16 or f16, each its own.  A token outside ``[0, vocabulary)`` gets a row of zeros and is
+    recorded in the device status word, so a synchronising launcher raises."""
+    _all_traced((tokens, table, out), "embedding")
+    _embedding_operands(tokens, table, out, "embedding", "out")
+    require_builder().emit_void("embedding", tokens, table, out, attrs={"scale": float(scale)})
+    return out
+
+
+def embedding_backward(grad_out: Any, tokens: Any, grad_table: Any, *, scale: float = 1.0, padding_token: int | None = None,
+                       accumulate: bool = False) -> Any:
+    """The gradient of ``embedding``: row ``v`` of ``grad_table`` is ``scale`` times the sum of the rows of ``grad_out`` whose
+    token is ``v``, added up in 32 bits in a fixed order (the same call gives the same bits) and rounded once.
+
+    Without ``accumulate`` the whole table is written, zeros where no token points; with it the sums are added to the
+    rows that tokens name and every other row is left alone.  ``padding_token`` contributes nothing.  A token outside
+    ``[0, vocabulary)`` contributes nothing either and is recorded in the device status word."""
+    _all_traced((grad_out, tokens, grad_table), "embedding_backward")
+    _embedding_operands(tokens, grad_table, grad_out, "embedding_backward", "grad_out")
+    vocabulary = grad_table.spec.shape[0]
+    if padding_token is not None and not 0 <= int(padding_token) < vocabulary:
+        raise ValueError(f"baybridge.embedding_backward expects a padding_token in [0, {vocabulary}), got {padding_token}")
+    require_builder().emit_void(
+        "embedding_backward", grad_out, tokens, grad_table,
+        attrs={"scale": float(scale), "padding_token": None if padding_token is None else int(padding_token), "accumulate": bool(accumulate)},
+    )
+    return grad_table
+
+
+def _norm_operands(op: str, x: TensorValue, same: dict[str, Any], vectors: dict[str, Any], mean: TensorValue, rstd: TensorValue) -> None:
+    if x.ndim < 1:
+        raise ValueError(f"baybridge.{op} requires rank >= 1 tensors")
+    hidden, rows = x.spec.shape[-1], x.spec.shape[:-1] or (1,)
+    _float_tensor(x, op, "x")
+    for name, value in same.items():
+        if value is not None and (value.spec.shape != x.spec.shape or value.spec.dtype != x.spec.dtype):
+            raise ValueError(f"baybridge.{op} expects {name} like x ({x.spec.dtype} {x.spec.shape}), got {value.spec.dtype} {value.spec.shape}")
+    for name, value in (("mean", mean), ("rstd", rstd)):
+        if value.spec.shape != rows or value.spec.dtype != "f32":
+            raise ValueError(f"baybridge.{op} expects {name} f32 {rows}, got {value.spec.dtype} {value.spec.shape}")
+    kinds = {value.spec.dtype for value in vectors.values() if value is not None}
+    for name, value in vectors.items():
+        if value is not None and value.spec.shape != (hidden,):
+            raise ValueError(f"baybridge.{op} expects {name} shape {(hidden,)}, got {value.spec.shape}")
+    if len(kinds) != 1 or not kinds <= {x.spec.dtype, "f32"}:
+        raise ValueError(f"baybridge.{op} expects {', '.join(vectors)} of one dtype, x's or f32, got {sorted(kinds)}")
+
+
+def layernorm_forward(x: Any, out: Any, mean: Any, rstd: Any, weight: Any, bias: Any = None, *, residual: Any = None,
+                      out_resid: Any = None, epsilon: float = 1e-5) -> Any:
+    """LayerNorm over the last axis that keeps what its gradient needs.
+
+    ``s = x`` (``x + residual`` where given, stored to ``out_resid``); ``out = (s - mean) * rstd * weight + bias`` with the
+    mean and ``rstd = 1 / sqrt(variance + epsilon)`` of every row, both stored in f32 (shape ``x.shape[:-1]``).  Statistics and
+    products are 32-bit, each output is rounded once.  ``weight`` and ``bias`` are ``[hidden]``, of x's dtype or f32; ``bias``
+    may be left out."""
+    given = tuple(value for value in (x, out, mean, rstd, weight, bias, residual, out_resid) if value is not None)
+    _all_traced(given, "layernorm_forward")
+    if (residual is None) != (out_resid is None):
+        raise ValueError("baybridge.layernorm_forward takes residual and out_resid together or not at all")
+    _norm_operands("layernorm_forward", x, {"out": out, "residual": residual, "out_resid": out_resid},
+                   {"weight": weight, "bias": bias}, mean, rstd)
+    require_builder().emit_void(
+        "layernorm_forward", *given, attrs={"epsilon": float(epsilon), "bias": bias is not None, "residual": residual is not None})
+    return out
+
+
+def layernorm_backward(grad_out: Any, x: Any, mean: Any, rstd: Any, weight: Any, grad_x: Any, grad_weight: Any, grad_bias: Any = None,
+                       *, grad_resid: Any = None) -> Any:
+    """The gradients of ``layernorm_forward`` from its input ``x`` (its ``out_resid`` where a residual was added) and the
+    statistics that it stored.
+
+    With ``n = (x - mean) * rstd`` and ``g = grad_out * weight``: ``grad_x = rstd * (g - mean(g) - n * mean(g * n))``, plus
+    ``grad_resid`` where given (the gradient that reaches ``out_resid`` on its own way; the sum is the gradient of both x and
+    the residual); ``grad_weight = sum over rows of grad_out * n``; ``grad_bias = sum over rows of grad_out``.  Sums are
+    32-bit in a fixed order: the same call gives the same bits.  ``weight``, ``grad_weight`` and ``grad_bias`` are ``[hidden]``
+    and of one dtype, x's or f32."""
+    given = tuple(value for value in (grad_out, x, mean, rstd, weight, grad_x, grad_weight, grad_bias, grad_resid) if value is not None)
+    _all_traced(given, "layernorm_backward")
+    _norm_operands("layernorm_backward", x, {"grad_out": grad_out, "grad_x": grad_x, "grad_resid": grad_resid},
+                   {"weight": weight, "grad_weight": grad_weight, "grad_bias": grad_bias}, mean, rstd)
+    require_builder().emit_void("layernorm_backward", *given, attrs={"bias": grad_bias is not None, "residual": grad_resid is not None})
+    return grad_x
+
+
+def adamw(params: Any, grads: Any, exp_avgs: Any, exp_avg_sqs: Any, schedule: Any, *, masters: Any = None,
+          betas: tuple[float, float] = (0.9, 0.999), epsilon: float = 1e-8, weight_decay: Any = 0.01) -> Any:
+    """One AdamW step over many tensors, in place.
+
+    ``params``, ``grads``, ``exp_avgs``, ``exp_avg_sqs`` (and ``masters``) are lists of as many tensors, the i-th of each of one
+    shape.  ``schedule`` is an f32 tensor ``[learning rate, step, gradient factor]`` on the device (step counts from 1), so a
+    recorded step replays with whatever it holds then.  Per element, in 32 bits::
+
+        g = grad * factor
+        exp_avg = beta1 * exp_avg + (1 - beta1) * g;  exp_avg_sq = beta2 * exp_avg_sq + (1 - beta2) * g * g
+        p = p * (1 - rate * weight_decay) - rate * (exp_avg / (1 - beta1**step)) / (sqrt(exp_avg_sq / (1 - beta2**step)) + epsilon)
+
+    Moments (and masters) are f32; parameters are f32, bf16 or f16; a gradient has its parameter's dtype or f32.  With
+    ``masters`` the step is taken on the 32-bit copies and ``params`` receive them rounded; the parameters are not read.
+    ``weight_decay`` is one number or one per tensor.  No two of the tensors may overlap."""
+    lists = {"params": params, "grads": grads, "exp_avgs": exp_avgs, "exp_avg_sqs": exp_avg_sqs}
+    if masters is not None:
+        lists["masters"] = masters
+    lists = {name: tuple(value) if isinstance(value, (list, tuple)) else (value,) for name, value in lists.items()}
+    count = len(lists["params"])
+    if count == 0 or any(len(tensors) != count for tensors in lists.values()):
+        raise ValueError("baybridge.adamw expects lists of one length >= 1, got " + ", ".join(f"{len(t)} {n}" for n, t in lists.items()))
+    _all_traced(tuple(tensor for tensors in lists.values() for tensor in tensors) + (schedule,), "adamw")
+    for index in range(count):
+        param = lists["params"][index]
+        _float_tensor(param, "adamw", f"params[{index}]")
+        for name, tensors in lists.items():
+            spec = tensors[index].spec
+            allowed = (param.spec.dtype,) if name == "params" else (param.spec.dtype, "f32") if name == "grads" else ("f32",)
+            if spec.shape != param.spec.shape or spec.dtype not in allowed:
+                raise ValueError(f"baybridge.adamw expects {name}[{index}] of shape {param.spec.shape} and dtype {' or '.join(allowed)}, "
+                                 f"got {spec.dtype} {spec.shape}")
+    if schedule.spec.shape != (3,) or schedule.spec.dtype != "f32":
+        raise ValueError(f"baybridge.adamw expects schedule f32 (3,): rate, step, gradient factor; got {schedule.spec.dtype} {schedule.spec.shape}")
+    beta1, beta2 = (float(beta) for beta in betas)
+    if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0):
+        raise ValueError(f"baybridge.adamw expects betas in [0, 1), got {betas}")
+    if not float(epsilon) >= 0.0:
+        raise ValueError(f"baybridge.adamw expects epsilon >= 0, got {epsilon}")
+    decay = [float(item) for item in weight_decay] if isinstance(weight_decay, (list, tuple)) else [float(weight_decay)] * count
+    if len(decay) != count:
+        raise ValueError(f"baybridge.adamw expects one weight_decay or {count}, got {len(decay)}")
+    require_builder().emit_void(
+        "adamw", *(tensor for tensors in lists.values() for tensor in tensors), schedule,
+        attrs={"count": count, "masters": masters is not None, "betas": [beta1, beta2], "epsilon": float(epsilon), "weight_decay": decay})
+    return params

@@ -24,6 +24,7 @@ from .launch_state import recording
 from .portable_ir import Layout, row_major_stride
 from .scalar_types import (
     LOGICAL_NUMPY,
+    byte_width,
     cast_scalar_value,
     element_type,
     normalize_dtype_name,
@@ -375,6 +376,66 @@ def from_dlpack(value: Any, assumed_align: int | None = None, stream: Any | None
     )
 
 
+class TensorGroup:
+    """Many device tensors under one handle, for ops that take lists of tensors (``adamw``).
+
+    The members are checked once, here: CUDA tensors on one device, dense, no two sharing memory.  Calls then pass the
+    group's addresses as they are instead of walking a list, which is what a step over hundreds of tensors would
+    otherwise spend its host time on.  A group holds its members and never changes; where a tensor is replaced (a new
+    gradient buffer), make a new group."""
+
+    __slots__ = ("handles", "signature", "device_id", "addresses")
+
+    def __init__(self, tensors: Any):
+        import ctypes
+
+        handles = tuple(value if isinstance(value, TensorHandle) else from_dlpack(value) for value in tensors)
+        if not handles:
+            raise ValueError("a tensor group needs at least one tensor")
+        spans = []
+        for index, handle in enumerate(handles):
+            if int(handle.device_type) != DLPACK_CUDA:
+                raise BackendNotImplementedError(f"tensor group member {index} is not a CUDA tensor")
+            if not handle.is_contiguous:
+                raise BackendNotImplementedError(f"tensor group member {index} is not contiguous")
+            address = handle.data_ptr()
+            if not address:
+                raise TypeError(f"tensor group member {index} does not expose a usable data_ptr()")
+            numel = 1
+            for extent in handle.shape:
+                numel *= extent
+            spans.append((address, address + numel * byte_width(handle.dtype), index))
+        if len({int(handle.device_id) for handle in handles}) > 1:
+            raise BackendNotImplementedError("the members of a tensor group live on different devices")
+        ordered = sorted(spans)
+        for (_, stop, first), (start, _, second) in zip(ordered, ordered[1:]):
+            if start < stop:
+                raise ValueError(f"tensor group members {first} and {second} share memory")
+        self.handles = handles
+        self.device_id = int(handles[0].device_id)
+        self.signature = group_signature((handle.dtype, handle.shape) for handle in handles)
+        self.addresses = (ctypes.c_void_p * len(handles))(*(span[0] for span in spans))
+
+    def __len__(self) -> int:
+        return len(self.handles)
+
+    def __iter__(self):
+        return iter(self.handles)
+
+    def __getitem__(self, index: int) -> TensorHandle:
+        return self.handles[index]
+
+
+def group_signature(members: Any) -> str:
+    """The dtypes and shapes of a group's members as one string, which calls compare."""
+    return ";".join(f"{dtype}{tuple(shape)}" for dtype, shape in members)
+
+
+def tensor_group(tensors: Any) -> TensorGroup:
+    """One handle for a list of device tensors (DLPack exporters or ``TensorHandle`` values)."""
+    return TensorGroup(tensors)
+
+
 def _is_dlpack(value: Any) -> bool:
     return hasattr(value, "__dlpack__") and hasattr(value, "__dlpack_device__")
 
@@ -411,7 +472,7 @@ def infer_runtime_spec(value: Any) -> tuple[str, tuple[int, ...] | None]:
 
 def normalize_runtime_argument(value: Any, stream: Any | None = None) -> Any:
     """DLPack exporters → ``TensorHandle``, nested number lists → ``RuntimeTensor``, containers recursively."""
-    if isinstance(value, (RuntimeScalar, RuntimeTensor, TensorHandle)):
+    if isinstance(value, (RuntimeScalar, RuntimeTensor, TensorHandle, TensorGroup)):
         return value
     if _is_dlpack(value):
         return from_dlpack(value, stream=stream)

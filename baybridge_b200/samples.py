@@ -557,6 +557,47 @@ def build_zoo(cute) -> SimpleNamespace:
 
     zoo.layernorm_kernel = layernorm_kernel
 
+    def make_embedding(scale: float = 1.0):
+        @cute.kernel
+        def embedding_kernel(tokens: cute.Tensor, table: cute.Tensor, out: cute.Tensor):
+            cute.embedding(tokens, table, out, scale=scale)
+
+        return embedding_kernel
+
+    zoo.make_embedding = make_embedding
+
+    def make_embedding_backward(scale: float = 1.0, padding_token: int | None = None, accumulate: bool = False):
+        @cute.kernel
+        def embedding_backward_kernel(grad_out: cute.Tensor, tokens: cute.Tensor, grad_table: cute.Tensor):
+            cute.embedding_backward(grad_out, tokens, grad_table, scale=scale, padding_token=padding_token, accumulate=accumulate)
+
+        return embedding_backward_kernel
+
+    zoo.make_embedding_backward = make_embedding_backward
+
+    @cute.kernel
+    def layernorm_forward_kernel(x: cute.Tensor, out: cute.Tensor, mean: cute.Tensor, rstd: cute.Tensor, weight: cute.Tensor,
+                                 bias: cute.Tensor):
+        cute.layernorm_forward(x, out, mean, rstd, weight, bias)
+
+    zoo.layernorm_forward = layernorm_forward_kernel
+
+    @cute.kernel
+    def layernorm_backward_kernel(grad_out: cute.Tensor, x: cute.Tensor, mean: cute.Tensor, rstd: cute.Tensor, weight: cute.Tensor,
+                                  grad_x: cute.Tensor, grad_weight: cute.Tensor, grad_bias: cute.Tensor):
+        cute.layernorm_backward(grad_out, x, mean, rstd, weight, grad_x, grad_weight, grad_bias)
+
+    zoo.layernorm_backward = layernorm_backward_kernel
+
+    def make_adamw(**options):
+        @cute.kernel
+        def adamw_kernel(params, grads, exp_avgs, exp_avg_sqs, schedule: cute.Tensor):
+            cute.adamw(params, grads, exp_avgs, exp_avg_sqs, schedule, **options)
+
+        return adamw_kernel
+
+    zoo.make_adamw = make_adamw
+
     @cute.kernel
     def attention_full(q: cute.Tensor, k: cute.Tensor, v: cute.Tensor, out: cute.Tensor, lse: cute.Tensor):
         cute.attention(q, k, v, out, lse)

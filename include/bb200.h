@@ -305,6 +305,60 @@ int bb200_attention_fwd_gather(const void* q, const void* k, const void* v, void
                                float* const* lse_destinations, int destination_count, int batch_offset, int batch,
                                int seq, int heads, int kv_heads, int head_dim, int causal, void* stream);
 
+/* ---- a training step's operators (upstream has none of them) ------------------------------------------------------ */
+
+/* Status-word code of a lookup that met a token outside its table. */
+#define BB200_TOKEN_OUT_OF_RANGE 311
+
+/* out[t, :] = scale * table[tokens[t], :] for t < count; tokens i32 / i64, table [vocabulary, hidden], out [count, hidden]
+ * row-major, each bf16 / f16 / f32; computed in f32 and rounded once.  A token outside [0, vocabulary) gets a row of zeros
+ * and sets the device status word to BB200_TOKEN_OUT_OF_RANGE.  16-byte vectors where both row tensors are 16-byte
+ * aligned and hidden is a multiple of 8 (4 if both are f32), single elements otherwise.  No upstream counterpart. */
+int bb200_embedding(bb200_dtype table_dtype, bb200_dtype out_dtype, bb200_dtype token_dtype, const void* tokens, const void* table,
+                    void* out, size_t count, size_t vocabulary, size_t hidden, float scale, void* stream);
+
+/* grad_table[v, :] = scale * sum over t with tokens[t] = v of grad_out[t, :], for every v < vocabulary (rows that no token
+ * names become zero); with accumulate != 0 the sums are added to the rows that tokens name and other rows are not
+ * touched.  Tokens equal to padding_token (-1: none) contribute nothing; tokens outside [0, vocabulary) neither, and they
+ * set the status word as above.  Sums are f32 in an order fixed by the token positions: the same call gives the same
+ * bits.  The tokens are sorted in a workspace from the library's pool, taken and given back in stream order.  No upstream
+ * counterpart. */
+int bb200_embedding_backward(bb200_dtype grad_dtype, bb200_dtype table_dtype, bb200_dtype token_dtype, const void* grad_out,
+                             const void* tokens, void* grad_table, size_t count, size_t vocabulary, size_t hidden, float scale,
+                             int64_t padding_token, int accumulate, void* stream);
+
+/* s = x (+ residual, stored to out_resid); out = (s - mean) * rstd * weight + bias; mean and rstd = 1 / sqrt(var + epsilon)
+ * (biased variance) of every row are stored for the backward pass.  residual / out_resid are both given or both NULL,
+ * bias may be NULL.  x, residual, out, out_resid: [rows, hidden] row-major, bf16 / f16 / f32; weight, bias: [hidden], of that
+ * dtype or f32; hidden at most 32768 (16-bit) / 16384 (f32), any value and alignment (multiples of 16 bytes are faster).
+ * out_resid may be x or residual itself; no other output may share memory with another tensor.  f32 arithmetic, one
+ * rounding per output.  No upstream counterpart (upstream's LayerNorm keeps no statistics: src/baybridge/frontend.py:3754-3793). */
+int bb200_layernorm_forward(bb200_dtype dtype, bb200_dtype weight_dtype, const void* x, const void* residual, const void* weight,
+                            const void* bias, void* out, void* out_resid, float* mean, float* rstd, size_t rows, size_t hidden,
+                            float epsilon, void* stream);
+
+/* With n = (x - mean) * rstd and g = grad_out * weight: grad_x = rstd * (g - mean(g) - n * mean(g * n)) (+ grad_resid if not
+ * NULL); grad_weight = sum over rows of grad_out * n; grad_bias (if not NULL) = sum over rows of grad_out.  Shapes, dtypes
+ * and limits as above, grad_weight and grad_bias of the weight's dtype; no output may share memory with another tensor.
+ * The column sums run in a fixed order (the same call gives the same bits) through a workspace from the library's pool,
+ * taken and given back in stream order.  No upstream counterpart. */
+int bb200_layernorm_backward(bb200_dtype dtype, bb200_dtype weight_dtype, const void* grad_out, const void* x, const float* mean,
+                             const float* rstd, const void* weight, const void* grad_resid, void* grad_x, void* grad_weight,
+                             void* grad_bias, size_t rows, size_t hidden, void* stream);
+
+/* One AdamW step over `count` tensors, in place:
+ *   g = grad * factor;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g g;
+ *   p = p (1 - rate decay) - rate (m / (1 - beta1^step)) / (sqrt(v / (1 - beta2^step)) + epsilon)
+ * in f32.  The arrays are host arrays of `count` entries, read during the call; tensor i has numels[i] elements, its
+ * parameter is bf16 / f16 / f32 (param_dtypes[i]), its gradient alike or f32, its moments f32.  With `masters` (else NULL)
+ * the step is taken on the f32 copies and the parameters receive them rounded.  schedule: device array {rate, step,
+ * factor}, f32, step counted from 1; it is read when the kernel runs, so a recorded step replays with new values.  No two
+ * of the tensors may share memory (checked among the tensors of one index).  One launch per 512 tensors of a pair of
+ * dtypes.  No upstream counterpart. */
+int bb200_adamw(int count, const size_t* numels, const int* param_dtypes, const int* grad_dtypes, const float* weight_decays,
+                void* const* params, const void* const* grads, void* const* exp_avgs, void* const* exp_avg_sqs, void* const* masters,
+                const float* schedule, double beta1, double beta2, float epsilon, void* stream);
+
 /* Kernels with bounded device-side waits record a give-up in a per-device status word.  This
  * reads and clears it: *status_out = 0 if no wait timed out since the last call.  Synchronises
  * `stream` first.  No upstream counterpart (its generated kernels never wait on one another). */
