@@ -1,0 +1,298 @@
+// layernorm_forward.cu — LayerNorm for training, forward pass that keeps its statistics, sm_100a:
+//
+//   s = x (+ residual, stored);  out = (s - mean) * rstd * weight + bias;  mean, rstd = 1 / sqrt(variance + eps) per row, stored
+//
+// Bound by HBM bytes: x (and residual) are read once, out (and out_resid) written once.  fp32 throughout, one rounding per
+// output; the variance is the mean of squared differences from the mean, taken from registers, so a large mean costs no
+// precision.  A persistent CTA per SM walks groups of rows (bb200_rows.cuh): weight and bias stay in registers, rows are
+// copied ahead into shared memory, so the two sums of a row wait while the next rows are on their way.
+#include "bb200_rows.cuh"
+#include "layernorm_train.h"
+
+namespace bb200 {
+namespace {
+
+template <typename T> struct Forward {
+  const T* x;
+  const T* residual;  // null: none, and out_resid is null too
+  const void* weight;
+  const void* bias;  // null: none
+  T* out;
+  T* out_resid;
+  float* mean;
+  float* rstd;
+  size_t rows;
+  int hidden;
+  float epsilon;
+  bool wide;  // weight and bias are f32
+};
+
+template <typename T, typename Rows, bool RESIDUAL>
+__global__ void __launch_bounds__(kRowThreads, 1)
+norm_rows(const __grid_constant__ Forward<T> p) {
+  constexpr int PAIRS = Rows::PAIRS, LANES = Rows::LANES, GROUPS = Rows::GROUPS;
+  extern __shared__ __align__(16) unsigned char shared[];
+  __shared__ RowSums<LANES> scratch[GROUPS];
+  dependent_launch_prologue();
+  const int group = threadIdx.x / LANES, lane = threadIdx.x % LANES, barrier = group + 1;
+  const T* sources[RESIDUAL ? 2 : 1];
+  sources[0] = p.x;
+  if constexpr (RESIDUAL) sources[1] = p.residual;
+  Rows rows(shared, sources, p.rows, p.hidden, lane, group);
+  const size_t stride = (size_t)gridDim.x * GROUPS;
+  size_t row = (size_t)blockIdx.x * GROUPS + group;
+  rows.start(row, stride);
+  F2 weight[PAIRS], bias[PAIRS];
+  column_pairs<T>(rows, p.weight, p.wide, weight);
+  column_pairs<T>(rows, p.bias, p.wide, bias);
+  const float scale = 1.0f / (float)p.hidden;
+  int turn = 0;
+  // all groups of the CTA take the same number of turns, so every thread of a warp is there for the exchanges
+  for (size_t first = (size_t)blockIdx.x * GROUPS; first < p.rows; first += stride, row += stride, rows.next()) {
+    const bool active = row < p.rows;
+    rows.arrive(row, stride);
+    F2 s[PAIRS];
+    F2 sum2 = both(0.0f);
+    const size_t offset = row * (size_t)p.hidden;
+    if (active) {
+      rows.get(0, s);
+      if constexpr (RESIDUAL) {
+        F2 r[PAIRS];
+        rows.get(1, r);
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) s[i] = s[i] + r[i];
+        rows.put(p.out_resid + offset, s);
+      }
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) sum2 = sum2 + s[i];
+    }
+    const float mean = row_sum<LANES>(total(sum2), &scratch[group], turn, barrier) * scale;
+    F2 centred = both(0.0f);
+    if (active) {
+      const F2 minus_mean = both(-mean);
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) {
+        s[i] = s[i] + minus_mean;
+        if constexpr (Rows::kWholePairs) {
+          if (rows.column(i, 0) < p.hidden) centred = fma2(s[i], s[i], centred);
+        } else {
+          float low, high;
+          split(s[i], low, high);
+          const F2 kept = make_f2(rows.column(i, 0) < p.hidden ? low : 0.0f, rows.column(i, 1) < p.hidden ? high : 0.0f);
+          centred = fma2(kept, kept, centred);
+        }
+      }
+    }
+    const float variance = row_sum<LANES>(total(centred), &scratch[group], turn, barrier) * scale;
+    const float rstd = 1.0f / sqrtf(variance + p.epsilon);
+    if (active) {
+      if (lane == 0) {
+        p.mean[row] = mean;
+        p.rstd[row] = rstd;
+      }
+      const F2 r = both(rstd);
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) s[i] = fma2(s[i] * r, weight[i], bias[i]);
+      rows.put(p.out + offset, s);
+    }
+  }
+  copy_async_wait<0>();
+}
+
+// One row to a CTA, all of it in registers: rows too long for the kernel above (more than 2048 vectors).
+template <typename T, int THREADS, int VPT>
+__global__ void __launch_bounds__(THREADS)
+norm_long_rows(const __grid_constant__ Forward<T> p) {
+  constexpr int VEC = 16 / sizeof(T);
+  __shared__ RowSums<THREADS> scratch;
+  dependent_launch_prologue();
+  const size_t row = blockIdx.x, offset = row * (size_t)p.hidden;
+  const float scale = 1.0f / (float)p.hidden;
+  float s[VPT][VEC];
+  float sum = 0.0f;
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int c = (threadIdx.x + j * THREADS) * VEC;
+    if (c < p.hidden) {
+      const Pack<T, VEC> a = load_stream<T, VEC>(p.x + offset + c);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s[j][e] = Conv<float, T>::widen(a.v[e]);
+      if (p.residual) {
+        const Pack<T, VEC> b = load_stream<T, VEC>(p.residual + offset + c);
+        Pack<T, VEC> r;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          s[j][e] += Conv<float, T>::widen(b.v[e]);
+          r.v[e] = Conv<float, T>::narrow(s[j][e]);
+        }
+        store_stream<T, VEC>(p.out_resid + offset + c, r);
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) sum += s[j][e];
+    }
+  }
+  int turn = 0;
+  const float mean = row_sum<THREADS>(sum, &scratch, turn, 1) * scale;
+  float centred = 0.0f;
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    if ((threadIdx.x + j * THREADS) * VEC < p.hidden) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        s[j][e] -= mean;
+        centred = fmaf(s[j][e], s[j][e], centred);
+      }
+    }
+  }
+  const float rstd = 1.0f / sqrtf(row_sum<THREADS>(centred, &scratch, turn, 1) * scale + p.epsilon);
+  if (threadIdx.x == 0) {
+    p.mean[row] = mean;
+    p.rstd[row] = rstd;
+  }
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int c = (threadIdx.x + j * THREADS) * VEC;
+    if (c < p.hidden) {
+      Pack<T, VEC> o;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float w = p.wide ? static_cast<const float*>(p.weight)[c + e] : Conv<float, T>::widen(static_cast<const T*>(p.weight)[c + e]);
+        const float b = !p.bias ? 0.0f : p.wide ? static_cast<const float*>(p.bias)[c + e] : Conv<float, T>::widen(static_cast<const T*>(p.bias)[c + e]);
+        o.v[e] = Conv<float, T>::narrow(fmaf(s[j][e] * rstd, w, b));
+      }
+      store_stream<T, VEC>(p.out + offset + c, o);
+    }
+  }
+}
+
+// Tensors that do not start on a 16-byte boundary, and long rows of no whole vectors: element by element, the row kept in
+// shared memory as fp32.
+constexpr int kElementThreads = 256;
+template <typename T>
+__global__ void __launch_bounds__(kElementThreads)
+norm_rows_by_element(const __grid_constant__ Forward<T> p) {
+  extern __shared__ float row_values[];
+  __shared__ RowSums<kElementThreads> scratch;
+  dependent_launch_prologue();
+  const size_t row = blockIdx.x, offset = row * (size_t)p.hidden;
+  const float scale = 1.0f / (float)p.hidden;
+  int turn = 0;
+  float sum = 0.0f;
+#pragma unroll 4
+  for (int c = threadIdx.x; c < p.hidden; c += kElementThreads) {
+    float v = Conv<float, T>::widen(p.x[offset + c]);
+    if (p.residual) {
+      v += Conv<float, T>::widen(p.residual[offset + c]);
+      p.out_resid[offset + c] = Conv<float, T>::narrow(v);
+    }
+    row_values[c] = v;  // read back by this thread only
+    sum += v;
+  }
+  const float mean = row_sum<kElementThreads>(sum, &scratch, turn, 1) * scale;
+  float centred = 0.0f;
+  for (int c = threadIdx.x; c < p.hidden; c += kElementThreads) {
+    const float d = row_values[c] - mean;
+    centred = fmaf(d, d, centred);
+  }
+  const float rstd = 1.0f / sqrtf(row_sum<kElementThreads>(centred, &scratch, turn, 1) * scale + p.epsilon);
+  if (threadIdx.x == 0) {
+    p.mean[row] = mean;
+    p.rstd[row] = rstd;
+  }
+  for (int c = threadIdx.x; c < p.hidden; c += kElementThreads) {
+    const float w = p.wide ? static_cast<const float*>(p.weight)[c] : Conv<float, T>::widen(static_cast<const T*>(p.weight)[c]);
+    const float b = !p.bias ? 0.0f : p.wide ? static_cast<const float*>(p.bias)[c] : Conv<float, T>::widen(static_cast<const T*>(p.bias)[c]);
+    p.out[offset + c] = Conv<float, T>::narrow(fmaf((row_values[c] - mean) * rstd, w, b));
+  }
+}
+
+template <typename T, typename Rows, bool RESIDUAL> int launch_rows(const Forward<T>& p, cudaStream_t stream) {
+  const auto kernel = norm_rows<T, Rows, RESIDUAL>;
+  if (int status = check_runtime(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Rows::kBytes), "cudaFuncSetAttribute(layernorm_forward)"))
+    return status;
+  const size_t wanted = (p.rows + Rows::GROUPS - 1) / Rows::GROUPS, most = (size_t)multiprocessor_count();
+  launch_dependent(kernel, dim3((unsigned)(wanted < most ? wanted : most)), dim3(kRowThreads), (size_t)Rows::kBytes, stream, p);
+  return check_launch("layernorm_forward kernel launch");
+}
+
+template <typename T> int forward(const Forward<T>& p, bool aligned, cudaStream_t stream) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int nvec = p.hidden / VEC;
+  if (aligned && p.hidden % VEC == 0) {
+    // two vectors a thread: 16 (8 for f32) columns, whose weight and bias fit the registers beside the row
+#define BB200_VECTOR_ROWS(LANES, VPT)                                                              \
+  if (nvec <= (LANES) * (VPT))                                                                     \
+    return p.residual ? launch_rows<T, VectorRows<T, LANES, VPT, 2>, true>(p, stream) : launch_rows<T, VectorRows<T, LANES, VPT, 1>, false>(p, stream)
+    BB200_VECTOR_ROWS(4, 2);
+    BB200_VECTOR_ROWS(8, 2);
+    BB200_VECTOR_ROWS(16, 2);
+    BB200_VECTOR_ROWS(32, 2);
+    BB200_VECTOR_ROWS(64, 2);
+    BB200_VECTOR_ROWS(128, 2);
+    BB200_VECTOR_ROWS(256, 2);
+    BB200_VECTOR_ROWS(512, 2);
+    if constexpr (VEC == 4) BB200_VECTOR_ROWS(512, 4);
+#undef BB200_VECTOR_ROWS
+    if (nvec <= 2048) launch_dependent(norm_long_rows<T, 1024, 2>, dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
+    else launch_dependent(norm_long_rows<T, 1024, 4>, dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
+    return check_launch("layernorm_forward kernel launch");
+  }
+  if (aligned) {
+#define BB200_SHIFTED_ROWS(LANES, COLUMNS)                                                         \
+  if (p.hidden <= (LANES) * (COLUMNS))                                                             \
+    return p.residual ? launch_rows<T, ShiftedRows<T, LANES, COLUMNS, 2>, true>(p, stream) : launch_rows<T, ShiftedRows<T, LANES, COLUMNS, 1>, false>(p, stream)
+    BB200_SHIFTED_ROWS(32, 4);
+    BB200_SHIFTED_ROWS(32, 16);
+    BB200_SHIFTED_ROWS(64, 16);
+    BB200_SHIFTED_ROWS(128, 16);
+    BB200_SHIFTED_ROWS(256, 16);
+    BB200_SHIFTED_ROWS(512, 16);
+#undef BB200_SHIFTED_ROWS
+  }
+  const int smem = p.hidden * (int)sizeof(float);
+  if (smem > 48 * 1024) {
+    if (int status = check_runtime(cudaFuncSetAttribute(norm_rows_by_element<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 32768 * 4),
+                                   "cudaFuncSetAttribute(layernorm_forward)"))
+      return status;
+  }
+  launch_dependent(norm_rows_by_element<T>, dim3((unsigned)p.rows), dim3(kElementThreads), (size_t)smem, stream, p);
+  return check_launch("layernorm_forward kernel launch");
+}
+
+}  // namespace
+}  // namespace bb200
+
+using namespace bb200;
+
+extern "C" int bb200_layernorm_forward(bb200_dtype dtype, bb200_dtype weight_dtype, const void* x, const void* residual, const void* weight,
+                                       const void* bias, void* out, void* out_resid, float* mean, float* rstd, size_t rows, size_t hidden,
+                                       float epsilon, void* stream) {
+  if (!x || !weight || !out || !mean || !rstd) return fail(BB200_E_INVALID_ARGUMENT, "layernorm_forward: null tensor pointer");
+  if (!residual != !out_resid) return fail(BB200_E_INVALID_ARGUMENT, "layernorm_forward: residual and out_resid go together");
+  if (int status = check_norm("layernorm_forward", dtype, weight_dtype, rows, hidden)) return status;
+  const size_t size = dtype_bytes(dtype), weight_size = dtype_bytes(weight_dtype), row_bytes = rows * hidden * size;
+  bool aligned = true;
+  for (const void* p : {x, residual, static_cast<const void*>(out), static_cast<const void*>(out_resid)}) {
+    if (misaligned(p, size)) return fail(BB200_E_MISALIGNED, "layernorm_forward: a tensor is not aligned to its element size");
+    aligned = aligned && aligned16(p);
+  }
+  for (const void* p : {weight, bias})
+    if (misaligned(p, weight_size)) return fail(BB200_E_MISALIGNED, "layernorm_forward: a tensor is not aligned to its element size");
+  if (misaligned(mean, 4) || misaligned(rstd, 4)) return fail(BB200_E_MISALIGNED, "layernorm_forward: a tensor is not aligned to its element size");
+  // out_resid may be x or residual itself: every element is read by the thread that writes it
+  const Range written[] = {{out, row_bytes}, {mean, rows * 4}, {rstd, rows * 4}, {out_resid, row_bytes}};
+  const Range read[] = {{x == out_resid ? nullptr : x, row_bytes}, {residual == out_resid ? nullptr : residual, row_bytes},
+                        {weight, hidden * weight_size}, {bias, hidden * weight_size}};
+  if (clash(written, read) || overlap(out, row_bytes, x, row_bytes) || overlap(out, row_bytes, residual, row_bytes))
+    return fail(BB200_E_INVALID_ARGUMENT, "layernorm_forward: an output shares memory with another tensor");
+#define BB200_FORWARD(T)                                                                                                          \
+  forward<T>({static_cast<const T*>(x), static_cast<const T*>(residual), weight, bias, static_cast<T*>(out), static_cast<T*>(out_resid), \
+              mean, rstd, rows, (int)hidden, epsilon, weight_dtype == BB200_F32},                                                 \
+             aligned, static_cast<cudaStream_t>(stream))
+  switch (dtype) {
+    case BB200_BF16: return BB200_FORWARD(__nv_bfloat16);
+    case BB200_F16: return BB200_FORWARD(__half);
+    default: return BB200_FORWARD(float);
+  }
+#undef BB200_FORWARD
+}
