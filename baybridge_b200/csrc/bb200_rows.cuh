@@ -85,11 +85,11 @@ template <int N> __device__ __forceinline__ void copy_async_wait() { asm volatil
 // ---- sums over the LANES threads that share a row ---------------------------------------------------------------------
 // LANES is a power of two; up to 32 they are neighbours in a warp, above they are whole warps that meet at named barrier
 // `barrier`.  Every thread of the group receives the sums, the same bits in each.  `scratch`: the group's own, two
-// buffers of one F2 per warp, used in turn (`turn` = 0 or 1): a warp can write a buffer again only after every warp has
-// passed the barrier of the other one and so has read this one.
-template <int LANES> struct RowSums {
+// buffers of COUNT floats per warp, used in turn (`turn` = 0 or 1): a warp can write a buffer again only after every warp
+// has passed the barrier of the other one and so has read this one.
+template <int LANES, int COUNT> struct alignas(16) RowSums {
   static constexpr int kWarps = LANES <= 32 ? 1 : LANES / 32;
-  F2 buffer[2][kWarps < 2 ? 2 : kWarps];
+  float buffer[2][kWarps][COUNT];
 };
 
 template <int LANES> __device__ __forceinline__ void row_barrier(int barrier) {
@@ -97,97 +97,101 @@ template <int LANES> __device__ __forceinline__ void row_barrier(int barrier) {
   else asm volatile("bar.sync %0, %1;" ::"r"(barrier), "n"(LANES) : "memory");
 }
 
-template <int LANES> __device__ __forceinline__ float row_sum(float a, RowSums<LANES>* scratch, int& turn, int barrier) {
-#pragma unroll
-  for (int offset = (LANES < 32 ? LANES : 32) / 2; offset > 0; offset >>= 1) a += __shfl_xor_sync(0xffffffffu, a, offset);
-  if constexpr (LANES > 32) {
-    constexpr int WARPS = LANES / 32;
-    float* buffer = reinterpret_cast<float*>(scratch->buffer[turn]);
-    if ((threadIdx.x & 31) == 0) buffer[(threadIdx.x / 32) % WARPS] = a;
-    row_barrier<LANES>(barrier);
-    a = buffer[0];
-#pragma unroll
-    for (int w = 1; w < WARPS; ++w) a += buffer[w];
-    turn ^= 1;
-  }
-  return a;
-}
-
-// Two sums at once.  In a whole warp the first exchange leaves one sum in each half-warp, which halves the shuffles.
-template <int LANES> __device__ __forceinline__ void row_sums(float& a, float& b, RowSums<LANES>* scratch, int& turn, int barrier) {
+// COUNT (1, 2 or 4) sums at once.  In a whole warp the first exchanges leave a part of the sums to each half or quarter
+// of the lanes, so four sums cost six shuffles and not twenty.
+template <int LANES, int COUNT>
+__device__ __forceinline__ void row_sums(float (&v)[COUNT], RowSums<LANES, COUNT>* scratch, int& turn, int barrier) {
   if constexpr (LANES < 32) {
 #pragma unroll
     for (int offset = LANES / 2; offset > 0; offset >>= 1) {
-      a += __shfl_xor_sync(0xffffffffu, a, offset);
-      b += __shfl_xor_sync(0xffffffffu, b, offset);
+#pragma unroll
+      for (int k = 0; k < COUNT; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], offset);
     }
   } else {
     const int lane = threadIdx.x & 31;
-    const bool upper = lane & 16;
-    float kept = upper ? b : a;
-    kept += __shfl_xor_sync(0xffffffffu, upper ? a : b, 16);
+    float kept[COUNT];
 #pragma unroll
-    for (int offset = 8; offset > 0; offset >>= 1) kept += __shfl_xor_sync(0xffffffffu, kept, offset);
+    for (int k = 0; k < COUNT; ++k) kept[k] = v[k];
+    int offset = 16;
+#pragma unroll
+    for (int n = COUNT; n > 1; n >>= 1, offset >>= 1) {
+      const bool upper = lane & offset;
+#pragma unroll
+      for (int k = 0; k < n / 2; ++k) {
+        const float sent = upper ? kept[k] : kept[k + n / 2];
+        kept[k] = (upper ? kept[k + n / 2] : kept[k]) + __shfl_xor_sync(0xffffffffu, sent, offset);
+      }
+    }
+    float sum = kept[0];
+#pragma unroll
+    for (int o = 32 / COUNT / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    // lane k * (32 / COUNT) now holds sum k
+    constexpr int kEach = 32 / COUNT;
     if constexpr (LANES == 32) {
-      a = __shfl_sync(0xffffffffu, kept, 0);
-      b = __shfl_sync(0xffffffffu, kept, 16);
+#pragma unroll
+      for (int k = 0; k < COUNT; ++k) v[k] = COUNT == 1 ? sum : __shfl_sync(0xffffffffu, sum, k * kEach);
     } else {
       constexpr int WARPS = LANES / 32;
-      F2* buffer = scratch->buffer[turn];
-      if ((lane & 15) == 0) reinterpret_cast<float*>(buffer + (threadIdx.x / 32) % WARPS)[lane >> 4] = kept;
+      float(&buffer)[WARPS][COUNT] = scratch->buffer[turn];
+      if (lane % kEach == 0) buffer[(threadIdx.x / 32) % WARPS][lane / kEach] = sum;
       row_barrier<LANES>(barrier);
-      F2 sum = buffer[0];
+      static_assert(WARPS * COUNT <= 32, "one value to a lane");
+      sum = lane < WARPS * COUNT ? (&buffer[0][0])[lane] : 0.0f;  // lane w * COUNT + k: warp w's part of sum k
 #pragma unroll
-      for (int w = 1; w < WARPS; ++w) sum = sum + buffer[w];
-      split(sum, a, b);
+      for (int o = WARPS * COUNT / 2; o >= COUNT; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+#pragma unroll
+      for (int k = 0; k < COUNT; ++k) v[k] = __shfl_sync(0xffffffffu, sum, k);
       turn ^= 1;
     }
   }
 }
 
 // ---- the rows of TENSORS matrices, copied ahead --------------------------------------------------------------------------
-// THREADS threads in groups of LANES; a group walks its rows, and the next rows' bytes are on their way to shared memory
-// while one is worked on.  Both forms give a thread the same columns of every row, as PAIRS pairs, so it can keep what
-// belongs to columns (weights, sums over rows) in registers.  Bytes in flight per SM decide the depth: about 80 KB cover
-// the latency of HBM3e at its bandwidth (44 B/ns per SM, 1 to 2 us under load).
-constexpr int kRowThreads = 512;
-
-template <int STAGE_BYTES> constexpr int stages_for() {
-  constexpr int wanted = 1 + (80 * 1024 + STAGE_BYTES - 1) / STAGE_BYTES;
-  constexpr int most = 200 * 1024 / STAGE_BYTES;
-  return wanted > 6 ? 6 : wanted < 3 ? (most < 3 ? most : 3) : (wanted > most ? most : wanted);
+// THREADS threads in groups of LANES; a group takes ROWS rows a turn (row, row + GROUPS, ...), and the next turns' bytes are
+// on their way to shared memory while it works on one.  Both forms give a thread the same columns of every row, as PAIRS
+// pairs, so it can keep what belongs to columns (sums over rows) in registers.  Bytes in flight per SM decide the depth:
+// about 80 KB cover the latency of HBM3e at its bandwidth (44 B/ns per SM, 1 to 2 us under load).
+template <int STAGE_BYTES, int MOST_BYTES> constexpr int stages_for() {
+  constexpr int wanted = 1 + (80 * 1024 + STAGE_BYTES - 1) / STAGE_BYTES, most = MOST_BYTES / STAGE_BYTES, within = wanted > 6 ? 6 : wanted < 3 ? 3 : wanted;
+  static_assert(most >= 2, "two stages have to fit");
+  return within < most ? within : most;
 }
+
+// `wanted` rows a turn, or one where two stages of that many would not fit.
+constexpr int turn_rows(int wanted, int row_bytes, int most_bytes) { return wanted * row_bytes * 2 <= most_bytes ? wanted : 1; }
 
 // Rows of whole 16-byte vectors, 16-byte aligned.  Thread `lane` of a group owns the vectors lane, lane + LANES, ...; it
 // copies and reads them itself, so it waits for nothing but its own copies.
-template <typename T, int LANES_, int VPT, int TENSORS> struct VectorRows {
-  static constexpr bool kWholePairs = true;  // a pair is inside the row or past its end, never half
-  static constexpr int LANES = LANES_, VEC = 16 / sizeof(T), PAIRS = VPT * VEC / 2, GROUPS = kRowThreads / LANES;
-  static constexpr int kSlot = kRowThreads * VPT * 16, kStage = kSlot * TENSORS, STAGES = stages_for<kStage>(), kBytes = kStage * STAGES;
+template <typename T, int THREADS_, int LANES_, int VPT, int TENSORS, int ROWS_, int MOST_BYTES> struct VectorRows {
+  static constexpr int THREADS = THREADS_, LANES = LANES_, VEC = 16 / sizeof(T), PAIRS = VPT * VEC / 2, GROUPS = THREADS / LANES;
+  static constexpr int kSlot = THREADS * VPT * 16, ROWS = turn_rows(ROWS_, kSlot * TENSORS, MOST_BYTES), kStage = kSlot * TENSORS * ROWS, STAGES = stages_for<kStage, MOST_BYTES>(), kBytes = kStage * STAGES;
 
   unsigned char* shared;
   const T* tensors[TENSORS];
   size_t rows;
   int hidden, lane, stage;
 
-  __device__ __forceinline__ VectorRows(unsigned char* memory, const T* const (&sources)[TENSORS], size_t rows_, int hidden_, int lane_, int)
+  __device__ __forceinline__ VectorRows(unsigned char* memory, const T* const (&sources)[TENSORS], size_t rows_, int hidden_, int lane_, int, int)
       : shared(memory), rows(rows_), hidden(hidden_), lane(lane_), stage(0) {
 #pragma unroll
     for (int t = 0; t < TENSORS; ++t) tensors[t] = sources[t];
   }
-  __device__ __forceinline__ unsigned char* slot(int at, int tensor, int j) const {
-    return shared + at * kStage + tensor * kSlot + (j * kRowThreads + threadIdx.x) * 16;
+  __device__ __forceinline__ unsigned char* slot(int at, int r, int tensor, int j) const {
+    return shared + at * kStage + (r * TENSORS + tensor) * kSlot + (j * THREADS + threadIdx.x) * 16;
   }
   __device__ __forceinline__ int vector(int j) const { return lane + j * LANES; }
   __device__ __forceinline__ bool has(int j) const { return vector(j) * VEC < hidden; }
   __device__ __forceinline__ void fetch(size_t row, int at) {
-    if (row < rows) {
-      const size_t offset = row * (size_t)hidden;
 #pragma unroll
-      for (int j = 0; j < VPT; ++j) {
-        if (has(j)) {
+    for (int r = 0; r < ROWS; ++r) {
+      if (row + r * GROUPS < rows) {
+        const size_t offset = (row + r * GROUPS) * (size_t)hidden;
 #pragma unroll
-          for (int t = 0; t < TENSORS; ++t) copy_async_16(slot(at, t, j), tensors[t] + offset + vector(j) * VEC);
+        for (int j = 0; j < VPT; ++j) {
+          if (has(j)) {
+#pragma unroll
+            for (int t = 0; t < TENSORS; ++t) copy_async_16(slot(at, r, t, j), tensors[t] + offset + vector(j) * VEC);
+          }
         }
       }
     }
@@ -195,27 +199,29 @@ template <typename T, int LANES_, int VPT, int TENSORS> struct VectorRows {
   }
   __device__ __forceinline__ void start(size_t row, size_t stride) {
 #pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      if (!has(j)) {  // slots past the row's end are never copied to: zeros, so rows are read without a question
+        for (int at = 0; at < STAGES * ROWS * TENSORS; ++at)
+          *reinterpret_cast<uint4*>(shared + at * kSlot + (j * THREADS + threadIdx.x) * 16) = make_uint4(0, 0, 0, 0);
+      }
+    }
+#pragma unroll
     for (int at = 0; at < STAGES - 1; ++at) fetch(row + at * stride, at);
   }
-  // The row at hand has arrived, and a later one is on its way into the slots of the row before it.
+  // The turn's rows have arrived, and later ones are on their way into the slots of the turn before it.
   __device__ __forceinline__ void arrive(size_t row, size_t stride) {
     fetch(row + (STAGES - 1) * stride, stage == 0 ? STAGES - 1 : stage - 1);
     copy_async_wait<STAGES - 1>();
   }
   __device__ __forceinline__ void next() { stage = stage + 1 == STAGES ? 0 : stage + 1; }
 
-  // The row's pairs of one tensor; zeros past the row's end.
-  __device__ __forceinline__ void get(int tensor, F2 (&out)[PAIRS]) const {
+  // Pairs of one tensor's row; zeros past the row's end.
+  __device__ __forceinline__ void get(int r, int tensor, F2 (&out)[PAIRS]) const {
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-      if (has(j)) {
-        const Pack<T, VEC> v = *reinterpret_cast<const Pack<T, VEC>*>(slot(stage, tensor, j));
+      const Pack<T, VEC> v = *reinterpret_cast<const Pack<T, VEC>*>(slot(stage, r, tensor, j));
 #pragma unroll
-        for (int i = 0; i < VEC / 2; ++i) out[j * (VEC / 2) + i] = Pairs<T>::get(v, i);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC / 2; ++i) out[j * (VEC / 2) + i] = both(0.0f);
-      }
+      for (int i = 0; i < VEC / 2; ++i) out[j * (VEC / 2) + i] = Pairs<T>::get(v, i);
     }
   }
   __device__ __forceinline__ void put(T* row, const F2 (&in)[PAIRS]) const {
@@ -230,37 +236,43 @@ template <typename T, int LANES_, int VPT, int TENSORS> struct VectorRows {
     }
   }
   __device__ __forceinline__ int column(int pair, int half) const { return vector(pair / (VEC / 2)) * VEC + pair % (VEC / 2) * 2 + half; }
+  // `v` with what lies past the row's end left out
+  __device__ __forceinline__ F2 inside(int pair, F2 v) const { return F2{has(pair / (VEC / 2)) ? v.bits : 0ull}; }
 };
 
 // Rows of any width in tensors whose first element is 16-byte aligned: the group copies the 16-byte windows that cover the
 // row (the last one of a tensor only as far as the tensor goes), and thread `lane` owns the columns lane, lane + LANES, ...
-// The copies are other threads' too, so the group meets at its barrier before it reads a row.
-template <typename T, int LANES_, int COLUMNS, int TENSORS> struct ShiftedRows {
-  static constexpr bool kWholePairs = false;
-  static constexpr int LANES = LANES_, PAIRS = COLUMNS / 2, GROUPS = kRowThreads / LANES;
-  static constexpr int kSlot = LANES * COLUMNS * (int)sizeof(T) + 32, kStage = kSlot * GROUPS * TENSORS, STAGES = stages_for<kStage>(),
-                       kBytes = kStage * STAGES;
+// The copies are other threads' too, so the group meets at its barrier before it reads a row.  SURE: so many of a thread's
+// columns lie inside every row that this form is used for (LANES * SURE <= hidden), and are not asked about.
+template <typename T, int THREADS_, int LANES_, int COLUMNS, int SURE, int TENSORS, int ROWS_, int MOST_BYTES> struct ShiftedRows {
+  static constexpr int THREADS = THREADS_, LANES = LANES_, PAIRS = COLUMNS / 2, GROUPS = THREADS / LANES;
+  static constexpr int kSlot = LANES * COLUMNS * (int)sizeof(T) + 32, ROWS = turn_rows(ROWS_, kSlot * TENSORS * GROUPS, MOST_BYTES), kGroup = kSlot * TENSORS * ROWS, kStage = kGroup * GROUPS,
+                       STAGES = stages_for<kStage, MOST_BYTES>(), kBytes = kStage * STAGES;
 
   unsigned char* shared;
   const T* tensors[TENSORS];
-  size_t rows;
-  int hidden, lane, barrier, stage, shift;
+  size_t rows, row_at_hand;
+  int hidden, lane, barrier, stage;
 
-  __device__ __forceinline__ ShiftedRows(unsigned char* memory, const T* const (&sources)[TENSORS], size_t rows_, int hidden_, int lane_, int group)
-      : shared(memory + group * (kSlot * TENSORS)), rows(rows_), hidden(hidden_), lane(lane_), barrier(group + 1), stage(0), shift(0) {
+  __device__ __forceinline__ ShiftedRows(unsigned char* memory, const T* const (&sources)[TENSORS], size_t rows_, int hidden_, int lane_, int group,
+                                         int barrier_)
+      : shared(memory + group * kGroup), rows(rows_), row_at_hand(0), hidden(hidden_), lane(lane_), barrier(barrier_), stage(0) {
 #pragma unroll
     for (int t = 0; t < TENSORS; ++t) tensors[t] = sources[t];
   }
-  __device__ __forceinline__ unsigned char* slot(int at, int tensor) const { return shared + at * kStage + tensor * kSlot; }
+  __device__ __forceinline__ unsigned char* slot(int at, int r, int tensor) const { return shared + at * kStage + (r * TENSORS + tensor) * kSlot; }
   __device__ __forceinline__ void fetch(size_t row, int at) {
-    if (row < rows) {
-      const size_t begin = row * (size_t)hidden * sizeof(T), window = begin & ~(size_t)15, end = rows * (size_t)hidden * sizeof(T);
-      const int vectors = (int)((begin - window + (size_t)hidden * sizeof(T) + 15) / 16);
-      for (int v = lane; v < vectors; v += LANES) {
-        const size_t from = window + (size_t)v * 16;
-        const uint32_t bytes = end - from < 16 ? (uint32_t)(end - from) : 16;
 #pragma unroll
-        for (int t = 0; t < TENSORS; ++t) copy_async_part(slot(at, t) + v * 16, reinterpret_cast<const unsigned char*>(tensors[t]) + from, bytes);
+    for (int r = 0; r < ROWS; ++r) {
+      if (row + r * GROUPS < rows) {
+        const size_t begin = (row + r * GROUPS) * (size_t)hidden * sizeof(T), window = begin & ~(size_t)15, end = rows * (size_t)hidden * sizeof(T);
+        const int vectors = (int)((begin - window + (size_t)hidden * sizeof(T) + 15) / 16);
+        for (int v = lane; v < vectors; v += LANES) {
+          const size_t from = window + (size_t)v * 16;
+          const uint32_t bytes = end - from < 16 ? (uint32_t)(end - from) : 16;
+#pragma unroll
+          for (int t = 0; t < TENSORS; ++t) copy_async_part(slot(at, r, t) + v * 16, reinterpret_cast<const unsigned char*>(tensors[t]) + from, bytes);
+        }
       }
     }
     copy_async_commit();
@@ -271,18 +283,18 @@ template <typename T, int LANES_, int COLUMNS, int TENSORS> struct ShiftedRows {
   }
   __device__ __forceinline__ void arrive(size_t row, size_t stride) {
     copy_async_wait<STAGES - 2>();
-    row_barrier<LANES>(barrier);  // everyone's copies have landed, and everyone is done with the row before
+    row_barrier<LANES>(barrier);  // everyone's copies have landed, and everyone is done with the turn before
     fetch(row + (STAGES - 1) * stride, stage == 0 ? STAGES - 1 : stage - 1);
-    shift = (int)((row * (size_t)hidden * sizeof(T)) & 15) / (int)sizeof(T);
+    row_at_hand = row;
   }
   __device__ __forceinline__ void next() { stage = stage + 1 == STAGES ? 0 : stage + 1; }
 
-  __device__ __forceinline__ void get(int tensor, F2 (&out)[PAIRS]) const {
-    const T* row = reinterpret_cast<const T*>(slot(stage, tensor)) + shift;
+  __device__ __forceinline__ void get(int r, int tensor, F2 (&out)[PAIRS]) const {
+    const int shift = (int)(((row_at_hand + r * GROUPS) * (size_t)hidden * sizeof(T)) & 15);
+    const T* row = reinterpret_cast<const T*>(slot(stage, r, tensor) + shift);
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) {
-      const int low = column(i, 0), high = column(i, 1);
-      out[i] = make_f2(low < hidden ? Conv<float, T>::widen(row[low]) : 0.0f, high < hidden ? Conv<float, T>::widen(row[high]) : 0.0f);
+      out[i] = make_f2(has(2 * i) ? Conv<float, T>::widen(row[column(i, 0)]) : 0.0f, has(2 * i + 1) ? Conv<float, T>::widen(row[column(i, 1)]) : 0.0f);
     }
   }
   __device__ __forceinline__ void put(T* row, const F2 (&in)[PAIRS]) const {
@@ -290,11 +302,19 @@ template <typename T, int LANES_, int COLUMNS, int TENSORS> struct ShiftedRows {
     for (int i = 0; i < PAIRS; ++i) {
       float low, high;
       split(in[i], low, high);
-      if (column(i, 0) < hidden) row[column(i, 0)] = Conv<float, T>::narrow(low);
-      if (column(i, 1) < hidden) row[column(i, 1)] = Conv<float, T>::narrow(high);
+      if (has(2 * i)) row[column(i, 0)] = Conv<float, T>::narrow(low);
+      if (has(2 * i + 1)) row[column(i, 1)] = Conv<float, T>::narrow(high);
     }
   }
   __device__ __forceinline__ int column(int pair, int half) const { return lane + (2 * pair + half) * LANES; }
+  __device__ __forceinline__ bool has(int k) const { return k < SURE || lane + k * LANES < hidden; }
+  // `v` with what lies past the row's end left out
+  __device__ __forceinline__ F2 inside(int pair, F2 v) const {
+    if (2 * pair + 1 < SURE) return v;
+    float low, high;
+    split(v, low, high);
+    return make_f2(has(2 * pair) ? low : 0.0f, has(2 * pair + 1) ? high : 0.0f);
+  }
 };
 
 // A vector over the columns, of the rows' type or f32: its pairs for this thread, zeros past the row's end.

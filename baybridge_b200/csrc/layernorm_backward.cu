@@ -27,19 +27,21 @@ template <typename T> struct Backward {
   bool wide;  // weight and the column sums are f32
 };
 
+constexpr int kRowThreads = 512, kMostSmem = 204800;
+
 template <typename T, typename Rows, bool RESIDUAL>
 __global__ void __launch_bounds__(kRowThreads, 1)
 norm_backward_rows(const __grid_constant__ Backward<T> p) {
   constexpr int PAIRS = Rows::PAIRS, LANES = Rows::LANES, GROUPS = Rows::GROUPS;
   extern __shared__ __align__(16) unsigned char shared[];
-  __shared__ RowSums<LANES> scratch[GROUPS];
+  __shared__ RowSums<LANES, 2> scratch[GROUPS];
   dependent_launch_prologue();
   const int group = threadIdx.x / LANES, lane = threadIdx.x % LANES, barrier = group + 1;
   const T* sources[RESIDUAL ? 3 : 2];
   sources[0] = p.grad_out;
   sources[1] = p.x;
   if constexpr (RESIDUAL) sources[2] = p.grad_resid;
-  Rows rows(shared, sources, p.rows, p.hidden, lane, group);
+  Rows rows(shared, sources, p.rows, p.hidden, lane, group, barrier);
   const size_t stride = (size_t)gridDim.x * GROUPS;
   size_t row = (size_t)blockIdx.x * GROUPS + group;
   rows.start(row, stride);
@@ -58,13 +60,14 @@ norm_backward_rows(const __grid_constant__ Backward<T> p) {
     rows.arrive(row, stride);
     F2 g[PAIRS], n[PAIRS];
     F2 sum_g = both(0.0f), sum_gn = both(0.0f);
+    const F2 factor = both(rstd);
     if (active) {
-      rows.get(0, g);
-      rows.get(1, n);
-      const F2 minus_mean = both(-mean), r = both(rstd);
+      rows.get(0, 0, g);
+      rows.get(0, 1, n);
+      const F2 minus_mean = both(-mean);
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {
-        n[i] = (n[i] + minus_mean) * r;
+        n[i] = (n[i] + minus_mean) * factor;
         grad_weight[i] = fma2(g[i], n[i], grad_weight[i]);
         grad_bias[i] = grad_bias[i] + g[i];
         g[i] = g[i] * weight[i];
@@ -72,18 +75,19 @@ norm_backward_rows(const __grid_constant__ Backward<T> p) {
         sum_gn = fma2(g[i], n[i], sum_gn);
       }
     }
-    float all_g = total(sum_g), all_gn = total(sum_gn);
-    row_sums<LANES>(all_g, all_gn, &scratch[group], turn, barrier);
+    float sums[2] = {total(sum_g), total(sum_gn)};
+    row_sums<LANES>(sums, &scratch[group], turn, barrier);
     if (active) {
-      const F2 minus_mean_g = both(-all_g * scale), minus_mean_gn = both(-all_gn * scale), r = both(rstd);
-      if constexpr (RESIDUAL) {
-        F2 resid[PAIRS];
-        rows.get(2, resid);
+      const F2 minus_mean_g = both(-sums[0] * scale), minus_mean_gn = both(-sums[1] * scale);
 #pragma unroll
-        for (int i = 0; i < PAIRS; ++i) g[i] = fma2(fma2(n[i], minus_mean_gn, g[i] + minus_mean_g), r, resid[i]);
+      for (int i = 0; i < PAIRS; ++i) g[i] = fma2(n[i], minus_mean_gn, g[i] + minus_mean_g);
+      if constexpr (RESIDUAL) {
+        rows.get(0, 2, n);
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) g[i] = fma2(g[i], factor, n[i]);
       } else {
 #pragma unroll
-        for (int i = 0; i < PAIRS; ++i) g[i] = fma2(n[i], minus_mean_gn, g[i] + minus_mean_g) * r;
+        for (int i = 0; i < PAIRS; ++i) g[i] = g[i] * factor;
       }
       rows.put(p.grad_x + row * (size_t)p.hidden, g);
     }
@@ -147,7 +151,7 @@ template <typename T> __device__ __forceinline__ float weight_at(const Backward<
 template <typename T>
 __global__ void __launch_bounds__(kElementThreads)
 norm_backward_by_element(const __grid_constant__ Backward<T> p) {
-  __shared__ RowSums<kElementThreads> scratch;
+  __shared__ RowSums<kElementThreads, 2> scratch;
   dependent_launch_prologue();
   const size_t row = blockIdx.x, offset = row * (size_t)p.hidden;
   const float mean = p.mean[row], rstd = p.rstd[row], scale = 1.0f / (float)p.hidden;
@@ -159,8 +163,9 @@ norm_backward_by_element(const __grid_constant__ Backward<T> p) {
     sum_gn = fmaf(g, (Conv<float, T>::widen(p.x[offset + c]) - mean) * rstd, sum_gn);
   }
   int turn = 0;
-  row_sums<kElementThreads>(sum_g, sum_gn, &scratch, turn, 1);
-  const float mean_g = sum_g * scale, mean_gn = sum_gn * scale;
+  float sums[2] = {sum_g, sum_gn};
+  row_sums<kElementThreads>(sums, &scratch, turn, 1);
+  const float mean_g = sums[0] * scale, mean_gn = sums[1] * scale;
 #pragma unroll 4
   for (int c = threadIdx.x; c < p.hidden; c += kElementThreads) {
     const float g = Conv<float, T>::widen(p.grad_out[offset + c]) * weight_at(p, c);
@@ -252,8 +257,8 @@ template <typename T> int backward(Backward<T> p, bool aligned, void* grad_weigh
     // two vectors a thread (16 columns, 8 for f32): weight, both column sums and the row's two products fit the registers
 #define BB200_VECTOR_ROWS(LANES, VPT)                                                                                  \
   if (nvec <= (LANES) * (VPT))                                                                                         \
-    return p.grad_resid ? launch_rows<T, VectorRows<T, LANES, VPT, 3>, true>(p, grad_weight, grad_bias, stream)        \
-                        : launch_rows<T, VectorRows<T, LANES, VPT, 2>, false>(p, grad_weight, grad_bias, stream)
+    return p.grad_resid ? launch_rows<T, VectorRows<T, kRowThreads, LANES, VPT, 3, 1, kMostSmem>, true>(p, grad_weight, grad_bias, stream)        \
+                        : launch_rows<T, VectorRows<T, kRowThreads, LANES, VPT, 2, 1, kMostSmem>, false>(p, grad_weight, grad_bias, stream)
     BB200_VECTOR_ROWS(4, 2);
     BB200_VECTOR_ROWS(8, 2);
     BB200_VECTOR_ROWS(16, 2);
@@ -265,16 +270,17 @@ template <typename T> int backward(Backward<T> p, bool aligned, void* grad_weigh
     if constexpr (VEC == 4) BB200_VECTOR_ROWS(512, 4);
 #undef BB200_VECTOR_ROWS
   } else if (aligned) {
-#define BB200_SHIFTED_ROWS(LANES, COLUMNS)                                                                             \
+#define BB200_SHIFTED_ROWS(LANES, COLUMNS, SURE)                                                                           \
   if (p.hidden <= (LANES) * (COLUMNS))                                                                                 \
-    return p.grad_resid ? launch_rows<T, ShiftedRows<T, LANES, COLUMNS, 3>, true>(p, grad_weight, grad_bias, stream)   \
-                        : launch_rows<T, ShiftedRows<T, LANES, COLUMNS, 2>, false>(p, grad_weight, grad_bias, stream)
-    BB200_SHIFTED_ROWS(32, 4);
-    BB200_SHIFTED_ROWS(32, 16);
-    BB200_SHIFTED_ROWS(64, 16);
-    BB200_SHIFTED_ROWS(128, 16);
-    BB200_SHIFTED_ROWS(256, 16);
-    BB200_SHIFTED_ROWS(512, 16);
+    return p.grad_resid ? launch_rows<T, ShiftedRows<T, kRowThreads, LANES, COLUMNS, SURE, 3, 1, kMostSmem>, true>(p, grad_weight, grad_bias, stream)   \
+                        : launch_rows<T, ShiftedRows<T, kRowThreads, LANES, COLUMNS, SURE, 2, 1, kMostSmem>, false>(p, grad_weight, grad_bias, stream)
+    BB200_SHIFTED_ROWS(32, 4, 0);
+    BB200_SHIFTED_ROWS(32, 8, 4);
+    BB200_SHIFTED_ROWS(32, 16, 8);
+    BB200_SHIFTED_ROWS(64, 16, 8);
+    BB200_SHIFTED_ROWS(128, 16, 8);
+    BB200_SHIFTED_ROWS(256, 16, 8);
+    BB200_SHIFTED_ROWS(512, 16, 8);
 #undef BB200_SHIFTED_ROWS
   }
   const size_t blocks = (p.hidden + kElementThreads - 1) / kElementThreads;

@@ -27,24 +27,38 @@ template <typename T> struct Forward {
   bool wide;  // weight and bias are f32
 };
 
+constexpr int kRowThreads = 1024;
+// Shared memory: the rows' slots, then weight and bias as f32, each thread's pairs where it reads them (pair i of lane l at
+// [i / 2][l][i % 2]: 16 bytes a lane, no bank conflict).
+template <typename Rows> constexpr int kVectorBytes = Rows::LANES * Rows::PAIRS * (int)sizeof(F2);
+
 template <typename T, typename Rows, bool RESIDUAL>
 __global__ void __launch_bounds__(kRowThreads, 1)
 norm_rows(const __grid_constant__ Forward<T> p) {
   constexpr int PAIRS = Rows::PAIRS, LANES = Rows::LANES, GROUPS = Rows::GROUPS;
   extern __shared__ __align__(16) unsigned char shared[];
-  __shared__ RowSums<LANES> scratch[GROUPS];
+  __shared__ RowSums<LANES, 1> scratch[GROUPS];
   dependent_launch_prologue();
-  const int group = threadIdx.x / LANES, lane = threadIdx.x % LANES, barrier = group + 1;
+  const int group = threadIdx.x / LANES, lane = threadIdx.x % LANES;  // a group's barrier is its own number
   const T* sources[RESIDUAL ? 2 : 1];
   sources[0] = p.x;
   if constexpr (RESIDUAL) sources[1] = p.residual;
-  Rows rows(shared, sources, p.rows, p.hidden, lane, group);
+  Rows rows(shared, sources, p.rows, p.hidden, lane, group, group);
   const size_t stride = (size_t)gridDim.x * GROUPS;
   size_t row = (size_t)blockIdx.x * GROUPS + group;
   rows.start(row, stride);
-  F2 weight[PAIRS], bias[PAIRS];
-  column_pairs<T>(rows, p.weight, p.wide, weight);
-  column_pairs<T>(rows, p.bias, p.wide, bias);
+  F2* weight = reinterpret_cast<F2*>(shared + Rows::kBytes);
+  F2* bias = weight + LANES * PAIRS;
+  if (group == 0) {
+    F2 v[PAIRS];
+    column_pairs<T>(rows, p.weight, p.wide, v);
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) weight[((i / 2) * LANES + lane) * 2 + i % 2] = v[i];
+    column_pairs<T>(rows, p.bias, p.wide, v);
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) bias[((i / 2) * LANES + lane) * 2 + i % 2] = v[i];
+  }
+  __syncthreads();
   const float scale = 1.0f / (float)p.hidden;
   int turn = 0;
   // all groups of the CTA take the same number of turns, so every thread of a warp is there for the exchanges
@@ -55,10 +69,10 @@ norm_rows(const __grid_constant__ Forward<T> p) {
     F2 sum2 = both(0.0f);
     const size_t offset = row * (size_t)p.hidden;
     if (active) {
-      rows.get(0, s);
+      rows.get(0, 0, s);
       if constexpr (RESIDUAL) {
         F2 r[PAIRS];
-        rows.get(1, r);
+        rows.get(0, 1, r);
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) s[i] = s[i] + r[i];
         rows.put(p.out_resid + offset, s);
@@ -66,25 +80,22 @@ norm_rows(const __grid_constant__ Forward<T> p) {
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) sum2 = sum2 + s[i];
     }
-    const float mean = row_sum<LANES>(total(sum2), &scratch[group], turn, barrier) * scale;
+    float sum[1] = {total(sum2)};
+    row_sums<LANES>(sum, &scratch[group], turn, group);
+    const float mean = sum[0] * scale;
     F2 centred = both(0.0f);
     if (active) {
       const F2 minus_mean = both(-mean);
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {
         s[i] = s[i] + minus_mean;
-        if constexpr (Rows::kWholePairs) {
-          if (rows.column(i, 0) < p.hidden) centred = fma2(s[i], s[i], centred);
-        } else {
-          float low, high;
-          split(s[i], low, high);
-          const F2 kept = make_f2(rows.column(i, 0) < p.hidden ? low : 0.0f, rows.column(i, 1) < p.hidden ? high : 0.0f);
-          centred = fma2(kept, kept, centred);
-        }
+        const F2 kept = rows.inside(i, s[i]);
+        centred = fma2(kept, kept, centred);
       }
     }
-    const float variance = row_sum<LANES>(total(centred), &scratch[group], turn, barrier) * scale;
-    const float rstd = 1.0f / sqrtf(variance + p.epsilon);
+    sum[0] = total(centred);
+    row_sums<LANES>(sum, &scratch[group], turn, group);
+    const float rstd = 1.0f / sqrtf(sum[0] * scale + p.epsilon);
     if (active) {
       if (lane == 0) {
         p.mean[row] = mean;
@@ -92,7 +103,12 @@ norm_rows(const __grid_constant__ Forward<T> p) {
       }
       const F2 r = both(rstd);
 #pragma unroll
-      for (int i = 0; i < PAIRS; ++i) s[i] = fma2(s[i] * r, weight[i], bias[i]);
+      for (int i = 0; i < PAIRS; i += 2) {
+        const int at = ((i / 2) * LANES + lane) * 2;
+        const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(weight + at), b = *reinterpret_cast<const ulonglong2*>(bias + at);
+        s[i] = fma2(s[i] * r, F2{w.x}, F2{b.x});
+        s[i + 1] = fma2(s[i + 1] * r, F2{w.y}, F2{b.y});
+      }
       rows.put(p.out + offset, s);
     }
   }
@@ -104,7 +120,7 @@ template <typename T, int THREADS, int VPT>
 __global__ void __launch_bounds__(THREADS)
 norm_long_rows(const __grid_constant__ Forward<T> p) {
   constexpr int VEC = 16 / sizeof(T);
-  __shared__ RowSums<THREADS> scratch;
+  __shared__ RowSums<THREADS, 1> scratch;
   dependent_launch_prologue();
   const size_t row = blockIdx.x, offset = row * (size_t)p.hidden;
   const float scale = 1.0f / (float)p.hidden;
@@ -132,7 +148,9 @@ norm_long_rows(const __grid_constant__ Forward<T> p) {
     }
   }
   int turn = 0;
-  const float mean = row_sum<THREADS>(sum, &scratch, turn, 1) * scale;
+  float sums[1] = {sum};
+  row_sums<THREADS>(sums, &scratch, turn, 1);
+  const float mean = sums[0] * scale;
   float centred = 0.0f;
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
@@ -144,7 +162,9 @@ norm_long_rows(const __grid_constant__ Forward<T> p) {
       }
     }
   }
-  const float rstd = 1.0f / sqrtf(row_sum<THREADS>(centred, &scratch, turn, 1) * scale + p.epsilon);
+  sums[0] = centred;
+  row_sums<THREADS>(sums, &scratch, turn, 1);
+  const float rstd = 1.0f / sqrtf(sums[0] * scale + p.epsilon);
   if (threadIdx.x == 0) {
     p.mean[row] = mean;
     p.rstd[row] = rstd;
@@ -172,7 +192,7 @@ template <typename T>
 __global__ void __launch_bounds__(kElementThreads)
 norm_rows_by_element(const __grid_constant__ Forward<T> p) {
   extern __shared__ float row_values[];
-  __shared__ RowSums<kElementThreads> scratch;
+  __shared__ RowSums<kElementThreads, 1> scratch;
   dependent_launch_prologue();
   const size_t row = blockIdx.x, offset = row * (size_t)p.hidden;
   const float scale = 1.0f / (float)p.hidden;
@@ -188,13 +208,17 @@ norm_rows_by_element(const __grid_constant__ Forward<T> p) {
     row_values[c] = v;  // read back by this thread only
     sum += v;
   }
-  const float mean = row_sum<kElementThreads>(sum, &scratch, turn, 1) * scale;
+  float sums[1] = {sum};
+  row_sums<kElementThreads>(sums, &scratch, turn, 1);
+  const float mean = sums[0] * scale;
   float centred = 0.0f;
   for (int c = threadIdx.x; c < p.hidden; c += kElementThreads) {
     const float d = row_values[c] - mean;
     centred = fmaf(d, d, centred);
   }
-  const float rstd = 1.0f / sqrtf(row_sum<kElementThreads>(centred, &scratch, turn, 1) * scale + p.epsilon);
+  sums[0] = centred;
+  row_sums<kElementThreads>(sums, &scratch, turn, 1);
+  const float rstd = 1.0f / sqrtf(sums[0] * scale + p.epsilon);
   if (threadIdx.x == 0) {
     p.mean[row] = mean;
     p.rstd[row] = rstd;
@@ -207,11 +231,12 @@ norm_rows_by_element(const __grid_constant__ Forward<T> p) {
 }
 
 template <typename T, typename Rows, bool RESIDUAL> int launch_rows(const Forward<T>& p, cudaStream_t stream) {
+  constexpr int kSmem = Rows::kBytes + 2 * kVectorBytes<Rows>;
   const auto kernel = norm_rows<T, Rows, RESIDUAL>;
-  if (int status = check_runtime(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Rows::kBytes), "cudaFuncSetAttribute(layernorm_forward)"))
+  if (int status = check_runtime(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem), "cudaFuncSetAttribute(layernorm_forward)"))
     return status;
   const size_t wanted = (p.rows + Rows::GROUPS - 1) / Rows::GROUPS, most = (size_t)multiprocessor_count();
-  launch_dependent(kernel, dim3((unsigned)(wanted < most ? wanted : most)), dim3(kRowThreads), (size_t)Rows::kBytes, stream, p);
+  launch_dependent(kernel, dim3((unsigned)(wanted < most ? wanted : most)), dim3(kRowThreads), (size_t)kSmem, stream, p);
   return check_launch("layernorm_forward kernel launch");
 }
 
@@ -219,10 +244,10 @@ template <typename T> int forward(const Forward<T>& p, bool aligned, cudaStream_
   constexpr int VEC = 16 / sizeof(T);
   const int nvec = p.hidden / VEC;
   if (aligned && p.hidden % VEC == 0) {
-    // two vectors a thread: 16 (8 for f32) columns, whose weight and bias fit the registers beside the row
+    // two vectors a thread, so that 1024 threads an SM fit the registers; weight and bias take 8 bytes a column of the memory
 #define BB200_VECTOR_ROWS(LANES, VPT)                                                              \
   if (nvec <= (LANES) * (VPT))                                                                     \
-    return p.residual ? launch_rows<T, VectorRows<T, LANES, VPT, 2>, true>(p, stream) : launch_rows<T, VectorRows<T, LANES, VPT, 1>, false>(p, stream)
+    return p.residual ? launch_rows<T, VectorRows<T, kRowThreads, LANES, VPT, 2, 1, 221184 - (LANES) * (VPT) * 16 / (int)sizeof(T) * 8>, true>(p, stream) : launch_rows<T, VectorRows<T, kRowThreads, LANES, VPT, 1, 1, 221184 - (LANES) * (VPT) * 16 / (int)sizeof(T) * 8>, false>(p, stream)
     BB200_VECTOR_ROWS(4, 2);
     BB200_VECTOR_ROWS(8, 2);
     BB200_VECTOR_ROWS(16, 2);
@@ -231,22 +256,25 @@ template <typename T> int forward(const Forward<T>& p, bool aligned, cudaStream_
     BB200_VECTOR_ROWS(128, 2);
     BB200_VECTOR_ROWS(256, 2);
     BB200_VECTOR_ROWS(512, 2);
-    if constexpr (VEC == 4) BB200_VECTOR_ROWS(512, 4);
+    if constexpr (VEC == 4) BB200_VECTOR_ROWS(1024, 2);
 #undef BB200_VECTOR_ROWS
     if (nvec <= 2048) launch_dependent(norm_long_rows<T, 1024, 2>, dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
     else launch_dependent(norm_long_rows<T, 1024, 4>, dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
     return check_launch("layernorm_forward kernel launch");
   }
   if (aligned) {
-#define BB200_SHIFTED_ROWS(LANES, COLUMNS)                                                         \
+#define BB200_SHIFTED_ROWS(LANES, COLUMNS, SURE)                                                       \
   if (p.hidden <= (LANES) * (COLUMNS))                                                             \
-    return p.residual ? launch_rows<T, ShiftedRows<T, LANES, COLUMNS, 2>, true>(p, stream) : launch_rows<T, ShiftedRows<T, LANES, COLUMNS, 1>, false>(p, stream)
-    BB200_SHIFTED_ROWS(32, 4);
-    BB200_SHIFTED_ROWS(32, 16);
-    BB200_SHIFTED_ROWS(64, 16);
-    BB200_SHIFTED_ROWS(128, 16);
-    BB200_SHIFTED_ROWS(256, 16);
-    BB200_SHIFTED_ROWS(512, 16);
+    return p.residual ? launch_rows<T, ShiftedRows<T, kRowThreads, LANES, COLUMNS, SURE, 2, 1, 221184 - (LANES) * (COLUMNS) * 8>, true>(p, stream) : launch_rows<T, ShiftedRows<T, kRowThreads, LANES, COLUMNS, SURE, 1, 1, 221184 - (LANES) * (COLUMNS) * 8>, false>(p, stream)
+    constexpr int kColumns = 2 * VEC;
+    BB200_SHIFTED_ROWS(32, 4, 0);
+    BB200_SHIFTED_ROWS(32, kColumns / 2, 4);
+    BB200_SHIFTED_ROWS(32, kColumns, kColumns / 2);
+    BB200_SHIFTED_ROWS(64, kColumns, kColumns / 2);
+    BB200_SHIFTED_ROWS(128, kColumns, kColumns / 2);
+    BB200_SHIFTED_ROWS(256, kColumns, kColumns / 2);
+    BB200_SHIFTED_ROWS(512, kColumns, kColumns / 2);
+    if constexpr (VEC == 4) BB200_SHIFTED_ROWS(1024, kColumns, kColumns / 2);
 #undef BB200_SHIFTED_ROWS
   }
   const int smem = p.hidden * (int)sizeof(float);
