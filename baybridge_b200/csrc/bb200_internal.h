@@ -19,9 +19,10 @@ inline int check_launch(const char* what) { return check_runtime(cudaGetLastErro
 
 // Launch `kernel` with programmatic stream serialisation: its CTAs may be placed while the kernel before it on `stream`
 // drains.  ONLY for kernels that run `dependent_launch_prologue()` (below) before their first global-memory access.
-// A capturing stream takes the ordinary launch.
+// A capturing stream takes the ordinary launch.  `cluster`: CTAs of a cluster along x.
 template <typename... Params, typename... Args>
-inline void launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, size_t dynamic_smem, cudaStream_t stream, Args... args) {
+inline void launch_dependent_cluster(void (*kernel)(Params...), dim3 grid, dim3 block, unsigned cluster, size_t dynamic_smem,
+                                     cudaStream_t stream, Args... args) {
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
   const bool capturing = cudaStreamIsCapturing(stream, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone;
   cudaLaunchConfig_t config = {};
@@ -29,14 +30,24 @@ inline void launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, s
   config.blockDim = block;
   config.dynamicSmemBytes = dynamic_smem;
   config.stream = stream;
-  cudaLaunchAttribute attribute = {};
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attributes[2] = {};
+  config.attrs = attributes;
   if (!capturing) {
-    config.attrs = &attribute;
-    config.numAttrs = 1;
+    attributes[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[config.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attributes[config.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attributes[config.numAttrs].val.clusterDim.x = cluster;
+    attributes[config.numAttrs].val.clusterDim.y = 1;
+    attributes[config.numAttrs++].val.clusterDim.z = 1;
   }
   cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);  // the caller reads the status with check_launch()
+}
+
+template <typename... Params, typename... Args>
+inline void launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, size_t dynamic_smem, cudaStream_t stream, Args... args) {
+  launch_dependent_cluster(kernel, grid, block, 1, dynamic_smem, stream, args...);
 }
 
 #ifdef __CUDACC__

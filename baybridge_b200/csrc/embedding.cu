@@ -8,13 +8,13 @@
 // fp32 and run in an order that the token positions alone fix, so the same call gives the same bits; no floating-point
 // atomics.  The gradient's steps:
 //
-//   1. a stable radix sort of (token, position) — one CTA in shared memory for up to 4096 tokens, else a histogram and
-//      a scatter launch per digit;
+//   1. a stable radix sort of (token, position) — one launch for up to 65536 tokens, held in the shared memory of a cluster
+//      of CTAs, else a histogram and a scatter launch per digit;
 //   2. segmented sums over equal chunks of the sorted positions, which balances frequent tokens by construction: a run
 //      of one token inside a chunk is written straight to its row, a run that crosses a chunk's border leaves an fp32
 //      partial row in the workspace;
-//   3. the partial rows of every crossing run are joined, in chunk order, and written;
-//   4. without `accumulate`, rows that no token names are filled with zeros.
+//   3. one launch that joins the partial rows of every crossing run and, without `accumulate`, fills the rows that no
+//      token names with zeros.
 //
 // Tokens outside [0, vocabulary) read as zeros (lookup) or contribute nothing (gradient) and are recorded in the device
 // status word.  A padding token and out-of-range tokens sort behind every row under the key `vocabulary`.
@@ -81,12 +81,13 @@ int launch_lookup(const void* tokens, const void* table, void* out, size_t count
 }
 
 // ---- sorting the tokens ---------------------------------------------------------------------------------------------
-// Least-significant-digit radix sort of (token, position), stable, digits of at most 9 bits.  A CTA ranks a tile of
-// 4096: warp w holds the tile's elements [256 w, 256 w + 256), 32 at a time in order; within 32 the rank among equal
-// digits comes from __match_any_sync, earlier 32s of the warp are counted in the warp's own shared-memory counters,
-// and earlier warps by a prefix over the sixteen counters of a digit.
-constexpr int kSortThreads = 512, kSortRounds = 8, kSortWarps = kSortThreads / 32, kTile = kSortThreads * kSortRounds, kDigitBits = 9,
-              kBins = 1 << kDigitBits;
+// Least-significant-digit radix sort of (token, position), stable, digits of at most 9 bits.  A CTA ranks 1024 * R elements:
+// warp w holds elements [32 R w, 32 R (w + 1)), 32 at a time in order; within 32 the rank among equal digits comes from
+// __match_any_sync, earlier 32s of the warp are counted in the warp's own shared-memory counters, and earlier warps by a
+// prefix over the 32 counters of a digit.
+constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kDigitBits = 9, kBins = 1 << kDigitBits;
+// 16-bit counters, two digits to a word; rows of 257 words keep the prefix over warps free of bank conflicts.
+constexpr int kCounterWords = kBins / 2 + 1;
 
 template <typename Id> __device__ __forceinline__ uint32_t key_of(Id raw, uint32_t vocabulary, long long padding, int* status_word) {
   const long long token = (long long)raw;
@@ -97,41 +98,56 @@ template <typename Id> __device__ __forceinline__ uint32_t key_of(Id raw, uint32
   return token == padding ? vocabulary : (uint32_t)token;
 }
 
-// Stable rank of each of a thread's eight elements among the tile's elements of the same digit; on return counters[d]
-// of warp 0 hold how many elements of the tile have digit d.  `counters`: [kSortWarps + 1][kBins].
-__device__ __forceinline__ void rank_tile(const uint32_t (&digit)[kSortRounds], uint32_t (&rank)[kSortRounds], uint32_t* counters) {
+// Stable rank of each of a thread's R elements among the CTA's elements of the same digit; totals[d] = how many there are.
+template <int R>
+__device__ __forceinline__ void rank_digits(const uint32_t (&digit)[R], uint32_t (&rank)[R], uint32_t (*counters)[kCounterWords], uint32_t* totals) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint32_t* mine = counters + warp * kBins;
-  for (int bin = lane; bin < kBins; bin += 32) mine[bin] = 0;
+  for (int word = lane; word < kCounterWords; word += 32) counters[warp][word] = 0;
+  uint16_t* mine = reinterpret_cast<uint16_t*>(counters[warp]);
   __syncwarp();
 #pragma unroll
-  for (int r = 0; r < kSortRounds; ++r) {
+  for (int r = 0; r < R; ++r) {
     const uint32_t same = __match_any_sync(0xffffffffu, digit[r]);
     const uint32_t before = __popc(same & ((1u << lane) - 1));
     rank[r] = mine[digit[r]] + before;
     __syncwarp();
-    if (before == 0) mine[digit[r]] += __popc(same);
+    if (before == 0) mine[digit[r]] = (uint16_t)(rank[r] + __popc(same));
     __syncwarp();
   }
   __syncthreads();
-  uint32_t total = 0;  // one thread per digit: exclusive prefix over the warps
-  if (threadIdx.x < kBins) {
+  {  // four threads to a word, eight warps to a thread: exclusive prefix over the warps, both halves of the word at once
+    const int word = threadIdx.x >> 2, part = threadIdx.x & 3;
+    static_assert(kSortThreads == kBins * 2 && kSortWarps == 32, "four threads to a word, eight warps each");
+    uint32_t n[8], sum = 0;
 #pragma unroll
-    for (int w = 0; w < kSortWarps; ++w) {
-      const uint32_t n = counters[w * kBins + threadIdx.x];
-      counters[w * kBins + threadIdx.x] = total;
-      total += n;
+    for (int w = 0; w < 8; ++w) n[w] = counters[part * 8 + w][word];
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const uint32_t own = n[w];
+      n[w] = sum;
+      sum += own;  // the halves stay below 8192
     }
-    counters[kSortWarps * kBins + threadIdx.x] = total;
+    uint32_t inclusive = sum;
+#pragma unroll
+    for (int offset = 1; offset < 4; offset <<= 1) {
+      const uint32_t below = __shfl_up_sync(0xffffffffu, inclusive, offset, 4);
+      if (part >= offset) inclusive += below;
+    }
+    const uint32_t base = inclusive - sum;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) counters[part * 8 + w][word] = base + n[w];
+    if (part == 3) {
+      totals[2 * word] = inclusive & 0xffffu;
+      totals[2 * word + 1] = inclusive >> 16;
+    }
   }
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kSortRounds; ++r) rank[r] += mine[digit[r]];
+  for (int r = 0; r < R; ++r) rank[r] += mine[digit[r]];
 }
 
-// Exclusive prefix sum over kBins values, one per thread (kBins == kSortThreads).
+// Exclusive prefix sum over kBins values, one to a thread (threads past them bring 0 and are ignored).
 __device__ __forceinline__ uint32_t exclusive_over_bins(uint32_t value, uint32_t* warp_totals) {
-  static_assert(kBins == kSortThreads, "one bin per thread");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t inclusive = value;
 #pragma unroll
@@ -141,63 +157,120 @@ __device__ __forceinline__ uint32_t exclusive_over_bins(uint32_t value, uint32_t
   }
   if (lane == 31) warp_totals[warp] = inclusive;
   __syncthreads();
-  uint32_t base = 0;
-  for (int w = 0; w < warp; ++w) base += warp_totals[w];
+  uint32_t others = lane < warp ? warp_totals[lane] : 0;
+#pragma unroll
+  for (int offset = 16; offset > 0; offset >>= 1) others += __shfl_xor_sync(0xffffffffu, others, offset);
   __syncthreads();
-  return base + inclusive - value;
+  return others + inclusive - value;
 }
 
-// Up to kTile tokens in one CTA: all digits in shared memory, one launch.
-template <typename Id>
-__global__ void __launch_bounds__(kSortThreads)
-sort_tokens_small(const Id* __restrict__ tokens, uint32_t count, uint32_t vocabulary, long long padding, int passes, int digit_bits,
-                  uint32_t* __restrict__ keys_out, uint32_t* __restrict__ order_out, uint8_t* __restrict__ named, int* status_word) {
-  extern __shared__ uint32_t shared[];
-  uint32_t* keys = shared;
-  uint32_t* order = keys + kTile;
-  uint32_t* counters = order + kTile;  // [kSortWarps + 1][kBins]
-  uint32_t* starts = counters + (kSortWarps + 1) * kBins;
-  __shared__ uint32_t warp_totals[kSortWarps];
+// Behind the sorted list stand a few keys that no row has, so that readers may look ahead of its end.
+constexpr int kListTail = 16;
+
+struct SortedList {
+  uint32_t* keys;
+  uint32_t* order;
+  uint32_t* crossings;  // [0]: how many runs cross a chunk's border (set to 0 here), then their first chunks
+};
+
+__device__ __forceinline__ void finish_list(const SortedList& list, uint32_t count, uint32_t vocabulary) {
+  if (blockIdx.x == 0 && threadIdx.x < kListTail) list.keys[count + threadIdx.x] = vocabulary;
+  if (blockIdx.x == 0 && threadIdx.x == kListTail) list.crossings[0] = 0;
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// The address of CTA `rank`'s copy of a shared variable of this CTA.
+__device__ __forceinline__ uint32_t in_cta(const void* shared, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(shared)), "r"(rank));
+  return a;
+}
+
+// Up to 65536 tokens in one launch: one cluster of 1, 2, 4 or 8 CTAs holds them all in shared memory.  Every pass ranks in
+// each CTA, adds up the CTAs' digit counts through distributed shared memory and sends every element to its place, the
+// last pass to global memory.
+template <int R> struct ClusterSort {
+  uint2 pairs[kSortThreads * R];
+  uint32_t counters[kSortWarps][kCounterWords];
+  uint32_t totals[kBins];
+  uint32_t starts[kBins];
+  uint32_t warp_totals[kSortWarps];
+};
+
+template <typename Id, int R>
+__global__ void __launch_bounds__(kSortThreads, 1)
+sort_in_cluster(const Id* __restrict__ tokens, uint32_t count, uint32_t vocabulary, long long padding, int passes, int digit_bits, uint32_t ctas,
+                const __grid_constant__ SortedList list, uint8_t* __restrict__ named, int* status_word) {
+  constexpr uint32_t kEach = kSortThreads * R;
+  extern __shared__ __align__(16) unsigned char shared[];
+  ClusterSort<R>& s = *reinterpret_cast<ClusterSort<R>*>(shared);
   dependent_launch_prologue();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint32_t key[kSortRounds], position[kSortRounds];
+  const uint32_t rank_of_cta = cluster_rank();
+  uint32_t key[R], position[R];
 #pragma unroll
-  for (int r = 0; r < kSortRounds; ++r) {
-    position[r] = warp * (32 * kSortRounds) + r * 32 + lane;
+  for (int r = 0; r < R; ++r) {
+    position[r] = rank_of_cta * kEach + warp * (32 * R) + r * 32 + lane;
+    // the fill beyond `count` sorts behind every token, dropped ones included, because it comes after them
     key[r] = position[r] < count ? key_of(tokens[position[r]], vocabulary, padding, status_word) : vocabulary;
     if (named && key[r] < vocabulary) named[key[r]] = 1;
   }
+  finish_list(list, count, vocabulary);
   for (int pass = 0; pass < passes; ++pass) {
-    uint32_t digit[kSortRounds], rank[kSortRounds];
+    uint32_t digit[R], rank[R];
 #pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) digit[r] = (key[r] >> (pass * digit_bits)) & (kBins - 1) & ((1u << digit_bits) - 1);
-    rank_tile(digit, rank, counters);
-    starts[threadIdx.x] = exclusive_over_bins(counters[kSortWarps * kBins + threadIdx.x], warp_totals);
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) {
-      const uint32_t at = starts[digit[r]] + rank[r];
-      keys[at] = key[r];
-      order[at] = position[r];
+    for (int r = 0; r < R; ++r) digit[r] = (key[r] >> (pass * digit_bits)) & ((1u << digit_bits) - 1);
+    rank_digits<R>(digit, rank, s.counters, s.totals);
+    uint32_t total = 0, earlier = 0;
+    if (ctas > 1) cluster_barrier();  // every CTA's totals stand
+    if (threadIdx.x < kBins) {
+      for (uint32_t c = 0; c < ctas; ++c) {
+        uint32_t n;
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(n) : "r"(in_cta(&s.totals[threadIdx.x], c)) : "memory");
+        if (c < rank_of_cta) earlier += n;
+        total += n;
+      }
     }
+    const uint32_t start = exclusive_over_bins(total, s.warp_totals) + earlier;
+    if (threadIdx.x < kBins) s.starts[threadIdx.x] = start;
     __syncthreads();
+    if (pass + 1 < passes) {
 #pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) {
-      const uint32_t at = warp * (32 * kSortRounds) + r * 32 + lane;
-      key[r] = keys[at];
-      position[r] = order[at];
+      for (int r = 0; r < R; ++r) {
+        const uint32_t to = s.starts[digit[r]] + rank[r];
+        asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(in_cta(&s.pairs[to % kEach], to / kEach)), "r"(key[r]), "r"(position[r]) : "memory");
+      }
+      if (ctas > 1) cluster_barrier();  // everything has arrived, and every CTA has read the totals
+      else __syncthreads();
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const uint2 pair = s.pairs[warp * (32 * R) + r * 32 + lane];
+        key[r] = pair.x;
+        position[r] = pair.y;
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const uint32_t to = s.starts[digit[r]] + rank[r];
+        if (to < count) {
+          list.keys[to] = key[r];
+          list.order[to] = position[r];
+        }
+      }
     }
-    __syncthreads();
   }
-#pragma unroll
-  for (int r = 0; r < kSortRounds; ++r) {  // the fill beyond `count` carries the last key and the last positions: it sorted behind
-    const uint32_t at = warp * (32 * kSortRounds) + r * 32 + lane;
-    if (at < count) {
-      keys_out[at] = key[r];
-      order_out[at] = position[r];
-    }
-  }
+  if (ctas > 1) cluster_barrier();  // nobody leaves while another CTA still reads its totals
 }
+
+// More tokens: per digit a launch that counts and a launch that scatters, a tile of 8192 to a CTA.
+constexpr int kTileRounds = 8, kTile = kSortThreads * kTileRounds;
 
 // counts[tile][digit] of one digit.  The first pass reads the tokens themselves and marks the rows they name.
 template <typename Id, bool FIRST>
@@ -206,10 +279,10 @@ count_digits(const Id* __restrict__ tokens, const uint32_t* __restrict__ keys, u
              int shift, uint32_t mask, uint32_t* __restrict__ counts, uint8_t* __restrict__ named, int* status_word) {
   __shared__ uint32_t local[kBins];
   dependent_launch_prologue();
-  local[threadIdx.x] = 0;
+  if (threadIdx.x < kBins) local[threadIdx.x] = 0;
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kSortRounds; ++r) {
+  for (int r = 0; r < kTileRounds; ++r) {
     const size_t at = (size_t)blockIdx.x * kTile + r * kSortThreads + threadIdx.x;
     if (at < count) {
       uint32_t key;
@@ -223,7 +296,7 @@ count_digits(const Id* __restrict__ tokens, const uint32_t* __restrict__ keys, u
     }
   }
   __syncthreads();
-  counts[(size_t)blockIdx.x * kBins + threadIdx.x] = local[threadIdx.x];
+  if (threadIdx.x < kBins) counts[(size_t)blockIdx.x * kBins + threadIdx.x] = local[threadIdx.x];
 }
 
 // Moves every element of the tile to its place by one digit.  The place of the tile's first element of a digit is the
@@ -233,24 +306,28 @@ template <typename Id, bool FIRST>
 __global__ void __launch_bounds__(kSortThreads)
 scatter_digits(const Id* __restrict__ tokens, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ order, uint32_t count,
                uint32_t vocabulary, long long padding, int shift, uint32_t mask, const uint32_t* __restrict__ counts, int tiles,
-               uint32_t* __restrict__ keys_out, uint32_t* __restrict__ order_out) {
-  __shared__ uint32_t counters[(kSortWarps + 1) * kBins];
+               const __grid_constant__ SortedList list, int last) {
+  __shared__ uint32_t counters[kSortWarps][kCounterWords];
+  __shared__ uint32_t totals[kBins];
   __shared__ uint32_t starts[kBins];
   __shared__ uint32_t warp_totals[kSortWarps];
   dependent_launch_prologue();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t total = 0, earlier = 0;
+  if (threadIdx.x < kBins) {
 #pragma unroll 8
-  for (int tile = 0; tile < tiles; ++tile) {
-    const uint32_t n = counts[(size_t)tile * kBins + threadIdx.x];
-    if (tile < (int)blockIdx.x) earlier += n;
-    total += n;
+    for (int tile = 0; tile < tiles; ++tile) {
+      const uint32_t n = counts[(size_t)tile * kBins + threadIdx.x];
+      if (tile < (int)blockIdx.x) earlier += n;
+      total += n;
+    }
   }
-  starts[threadIdx.x] = exclusive_over_bins(total, warp_totals) + earlier;
-  uint32_t key[kSortRounds], position[kSortRounds], digit[kSortRounds], rank[kSortRounds];
+  const uint32_t start = exclusive_over_bins(total, warp_totals) + earlier;
+  if (threadIdx.x < kBins) starts[threadIdx.x] = start;
+  uint32_t key[kTileRounds], position[kTileRounds], digit[kTileRounds], rank[kTileRounds];
 #pragma unroll
-  for (int r = 0; r < kSortRounds; ++r) {
-    const size_t at = (size_t)blockIdx.x * kTile + warp * (32 * kSortRounds) + r * 32 + lane;
+  for (int r = 0; r < kTileRounds; ++r) {
+    const size_t at = (size_t)blockIdx.x * kTile + warp * (32 * kTileRounds) + r * 32 + lane;
     const bool valid = at < count;  // only the last tile has elements that are not, and they rank behind its others
     if constexpr (FIRST) {
       key[r] = valid ? key_of(tokens[at], vocabulary, padding, static_cast<int*>(nullptr)) : vocabulary;
@@ -261,144 +338,165 @@ scatter_digits(const Id* __restrict__ tokens, const uint32_t* __restrict__ keys,
     }
     digit[r] = valid ? (key[r] >> shift) & mask : kBins - 1;
   }
-  rank_tile(digit, rank, counters);
+  rank_digits<kTileRounds>(digit, rank, counters, totals);
 #pragma unroll
-  for (int r = 0; r < kSortRounds; ++r) {
-    const size_t at = (size_t)blockIdx.x * kTile + warp * (32 * kSortRounds) + r * 32 + lane;
+  for (int r = 0; r < kTileRounds; ++r) {
+    const size_t at = (size_t)blockIdx.x * kTile + warp * (32 * kTileRounds) + r * 32 + lane;
     if (at < count) {
       const uint32_t to = starts[digit[r]] + rank[r];
-      keys_out[to] = key[r];
-      order_out[to] = position[r];
+      list.keys[to] = key[r];
+      list.order[to] = position[r];
     }
   }
+  if (last) finish_list(list, count, vocabulary);
 }
 
 // ---- segmented sums ---------------------------------------------------------------------------------------------------
-constexpr int kBatch = 8;  // rows of grad_out a thread has in flight
-
-template <typename W, int VEC> __device__ __forceinline__ void write_row(W* __restrict__ row, const float (&sum)[VEC], float scale, bool accumulate) {
+template <typename W, int VEC> __device__ __forceinline__ void write_row(W* __restrict__ row, const float (&sum)[VEC], float scale) {
   Pack<W, VEC> r;
-  if (accumulate) {
-    const Pack<W, VEC> old = load_stream<W, VEC>(row);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) r.v[e] = Conv<float, W>::narrow(fmaf(sum[e], scale, Conv<float, W>::widen(old.v[e])));
-  } else {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) r.v[e] = Conv<float, W>::narrow(sum[e] * scale);
-  }
+  for (int e = 0; e < VEC; ++e) r.v[e] = Conv<float, W>::narrow(sum[e] * scale);
   store_stream<W, VEC>(row, r);
+}
+template <typename W, int VEC>
+__device__ __forceinline__ void add_to_row(W* __restrict__ row, const Pack<W, VEC>& old, const float (&sum)[VEC], float scale) {
+  Pack<W, VEC> r;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) r.v[e] = Conv<float, W>::narrow(fmaf(sum[e], scale, Conv<float, W>::widen(old.v[e])));
+  store_stream<W, VEC>(row, r);
+}
+template <int VEC> __device__ __forceinline__ void keep_partial(float* to, const float (&sum)[VEC]) {
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) to[e] = sum[e];
 }
 
 struct Segments {
-  const uint32_t* keys;   // sorted tokens
+  const uint32_t* keys;   // sorted tokens, with a tail of keys that no row has
   const uint32_t* order;  // their positions
-  float* partial;         // [chunks][2][hidden]: the sums of a chunk's first run (it began before) and of its last (it goes on)
+  uint32_t* crossings;
+  float* partial;  // [chunks][2][hidden]: the sums of a chunk's first run (it began before) and of its last (it goes on)
   uint32_t count, vocabulary, chunk_length, chunks;
   int steps, lane_bits;
 };
 
-// One group of `1 << lane_bits` threads per chunk; a thread owns one vector column of it.
-template <typename G, typename W, int VEC>
+// One group of `1 << lane_bits` threads per chunk; a thread owns one vector column of it and has a batch of rows in
+// flight, with the table's rows that the batch completes where they are added to.
+template <typename G, typename W, int VEC, bool ADD>
 __global__ void __launch_bounds__(kThreads)
-sum_chunks(const __grid_constant__ Segments s, const G* __restrict__ grad_out, W* __restrict__ grad_table, float scale, int accumulate) {
+sum_chunks(const __grid_constant__ Segments s, const G* __restrict__ grad_out, W* __restrict__ grad_table, float scale) {
+  constexpr int kBatch = (int)sizeof(G) * VEC + (ADD ? (int)sizeof(W) * VEC : 0) <= 16 ? 8 : 4;
   dependent_launch_prologue();
   const size_t chunk = (size_t)blockIdx.x * (kThreads >> s.lane_bits) + (threadIdx.x >> s.lane_bits);
   if (chunk >= s.chunks) return;
+  const int lane = threadIdx.x & ((1 << s.lane_bits) - 1);
   const size_t hidden = (size_t)s.steps * VEC;
   const uint32_t first = (uint32_t)(chunk * s.chunk_length);
-  const uint32_t end = s.count - first < s.chunk_length ? s.count : first + s.chunk_length;
-  if (s.keys[first] >= s.vocabulary) return;  // only dropped tokens from here on
-  for (int step = (blockIdx.y << s.lane_bits) + (threadIdx.x & ((1 << s.lane_bits) - 1)); step < s.steps; step += gridDim.y << s.lane_bits) {
+  const bool first_began_before = first > 0 && s.keys[first - 1] == s.keys[first];
+  for (int step = (blockIdx.y << s.lane_bits) + lane; step < s.steps; step += gridDim.y << s.lane_bits) {
     const size_t column = (size_t)step * VEC;
-    uint32_t current = s.keys[first];
-    bool began_before = first > 0 && s.keys[first - 1] == current;
+    bool began_before = first_began_before, open = false;
     float sum[VEC] = {};
-    bool live = true;
-    for (uint32_t at = first; at < end && live; at += kBatch) {
-      uint32_t key[kBatch];
+    for (uint32_t at = first; at < first + s.chunk_length && at < s.count; at += kBatch) {
+      uint32_t key[kBatch + 1];
+#pragma unroll
+      for (int j = 0; j <= kBatch; ++j) key[j] = s.keys[at + j];  // chunks are whole batches, the list has a tail
+      if (key[0] >= s.vocabulary) break;                         // dropped tokens, or the tail: nothing follows
       Pack<G, VEC> rows[kBatch];
+      Pack<W, VEC> old[ADD ? kBatch : 1];
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
-        key[j] = at + j < end ? s.keys[at + j] : s.vocabulary;
-        if (key[j] < s.vocabulary) rows[j] = load_stream<G, VEC>(grad_out + (size_t)s.order[at + j] * hidden + column);
+        if (key[j] < s.vocabulary) {
+          rows[j] = load_stream<G, VEC>(grad_out + (size_t)s.order[at + j] * hidden + column);
+          if constexpr (ADD) {
+            if (key[j] != key[j + 1]) old[j] = load_stream<W, VEC>(grad_table + (size_t)key[j] * hidden + column);
+          }
+        }
       }
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
-        if (key[j] >= s.vocabulary) {  // behind the chunk's end, or dropped tokens: nothing follows
-          live = false;
-        } else {
-          if (key[j] != current) {
-            if (began_before) {
-              float* to = s.partial + (chunk * 2) * hidden + column;
-#pragma unroll
-              for (int e = 0; e < VEC; ++e) to[e] = sum[e];
-            } else {
-              write_row<W, VEC>(grad_table + (size_t)current * hidden + column, sum, scale, accumulate != 0);
-            }
-            current = key[j];
-            began_before = false;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) sum[e] = 0.0f;
-          }
+        if (key[j] < s.vocabulary) {
           float value[VEC];
           widen<G, VEC>(rows[j], value);
 #pragma unroll
           for (int e = 0; e < VEC; ++e) sum[e] += value[e];
+          open = key[j] == key[j + 1];
+          if (!open) {
+            W* row = grad_table + (size_t)key[j] * hidden + column;
+            if (began_before) keep_partial<VEC>(s.partial + chunk * 2 * hidden + column, sum);
+            else if constexpr (ADD) add_to_row<W, VEC>(row, old[j], sum, scale);
+            else write_row<W, VEC>(row, sum, scale);
+            began_before = false;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) sum[e] = 0.0f;
+          }
         }
       }
     }
-    const bool goes_on = end < s.count && s.keys[end] == current;
-    if (began_before || goes_on) {
-      float* to = s.partial + (chunk * 2 + (began_before ? 0 : 1)) * hidden + column;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) to[e] = sum[e];
-    } else {
-      write_row<W, VEC>(grad_table + (size_t)current * hidden + column, sum, scale, accumulate != 0);
+    if (open) {
+      keep_partial<VEC>(s.partial + (chunk * 2 + (began_before ? 0 : 1)) * hidden + column, sum);
+      if (!began_before && step == 0) s.crossings[1 + atomicAdd(s.crossings, 1u)] = (uint32_t)chunk;
     }
   }
 }
 
-// Joins the partial sums of every run that crosses a chunk's border; the chunk where the run begins does it.
-template <typename W, int VEC>
+// Two jobs in one launch.  The first `join_blocks` CTAs join the partial sums of the runs that cross a chunk's border: 32
+// vector columns of one run at a time, eight warps over its chunks, added up in a fixed order.  The other CTAs, where the
+// whole table is written, fill the rows that no token names with zeros; the joins hide behind them.
+template <typename W, int VEC, bool ADD>
 __global__ void __launch_bounds__(kThreads)
-join_chunks(const __grid_constant__ Segments s, W* __restrict__ grad_table, float scale, int accumulate) {
+join_and_fill(const __grid_constant__ Segments s, W* __restrict__ grad_table, float scale, unsigned join_blocks, const uint8_t* __restrict__ named) {
+  __shared__ float parts[kThreads / 32][32][VEC + 1];
   dependent_launch_prologue();
-  const size_t chunk = (size_t)blockIdx.x * (kThreads >> s.lane_bits) + (threadIdx.x >> s.lane_bits);
-  if (chunk + 1 >= s.chunks) return;  // the last chunk's last run ends with it
   const size_t hidden = (size_t)s.steps * VEC;
-  const uint32_t first = (uint32_t)(chunk * s.chunk_length), next = first + s.chunk_length;
-  const uint32_t key = s.keys[next - 1];
-  if (key >= s.vocabulary || s.keys[next] != key) return;
-  if (first > 0 && s.keys[first] == key && s.keys[first - 1] == key) return;  // began in an earlier chunk
-  // the last chunk that the run reaches into
-  size_t last = chunk + 1;
-  while (last + 1 < s.chunks && s.keys[(last + 1) * s.chunk_length] == key) ++last;
-  for (int step = (blockIdx.y << s.lane_bits) + (threadIdx.x & ((1 << s.lane_bits) - 1)); step < s.steps; step += gridDim.y << s.lane_bits) {
-    const size_t column = (size_t)step * VEC;
-    float sum[VEC];
+  if (blockIdx.x >= join_blocks) {
+    const size_t row = (size_t)(blockIdx.x - join_blocks) * (kThreads >> s.lane_bits) + (threadIdx.x >> s.lane_bits);
+    if (row >= s.vocabulary || named[row]) return;
+    Pack<W, VEC> zero;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) sum[e] = s.partial[(chunk * 2 + 1) * hidden + column + e];
-    for (size_t c = chunk + 1; c <= last; ++c) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) sum[e] += s.partial[c * 2 * hidden + column + e];
-    }
-    write_row<W, VEC>(grad_table + (size_t)key * hidden + column, sum, scale, accumulate != 0);
+    for (int e = 0; e < VEC; ++e) zero.v[e] = Conv<float, W>::narrow(0.0f);
+    const int lanes = 1 << s.lane_bits;
+    for (int step = threadIdx.x & (lanes - 1); step < s.steps; step += lanes) store_stream<W, VEC>(grad_table + (row * s.steps + step) * VEC, zero);
+    return;
   }
-}
-
-// Zeros for every row that no token names.
-template <typename W, int VEC>
-__global__ void __launch_bounds__(kThreads)
-zero_unnamed(const uint8_t* __restrict__ named, W* __restrict__ grad_table, uint32_t vocabulary, int steps, int lane_bits) {
-  dependent_launch_prologue();
-  const size_t row = (size_t)blockIdx.x * (kThreads >> lane_bits) + (threadIdx.x >> lane_bits);
-  if (row >= vocabulary || named[row]) return;
-  Pack<W, VEC> zero;
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  const uint32_t tiles = (uint32_t)(s.steps + 31) / 32;
+  const unsigned long long items = (unsigned long long)s.crossings[0] * tiles;
+  for (unsigned long long item = blockIdx.x; item < items; item += join_blocks) {
+    const size_t chunk = s.crossings[1 + item / tiles];
+    const int step = (int)(item % tiles) * 32 + lane;
+    const size_t column = (size_t)step * VEC;
+    const uint32_t key = s.keys[(chunk + 1) * s.chunk_length - 1];
+    size_t end = chunk + 1;  // one past the last chunk that the run reaches into: the chunks it does begin with the key
+    for (bool more = true; more; ) {
+      const size_t probe = end + threadIdx.x;
+      const int found = __syncthreads_count(probe < s.chunks && s.keys[probe * s.chunk_length] == key);
+      end += found;
+      more = found == kThreads;
+    }
+    float sum[VEC] = {};
+    if (step < s.steps) {
+#pragma unroll 4
+      for (size_t c = chunk + slice; c < end; c += kThreads / 32) {
+        const float* from = s.partial + (c * 2 + (c == chunk ? 1 : 0)) * hidden + column;
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) zero.v[e] = Conv<float, W>::narrow(0.0f);
-  const int lanes = 1 << lane_bits;
-  for (int step = threadIdx.x & (lanes - 1); step < steps; step += lanes)
-    store_stream<W, VEC>(grad_table + (row * steps + step) * VEC, zero);
+        for (int e = 0; e < VEC; ++e) sum[e] += from[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) parts[slice][lane][e] = sum[e];
+    __syncthreads();
+    if (slice == 0 && step < s.steps) {
+#pragma unroll
+      for (int w = 1; w < kThreads / 32; ++w) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sum[e] += parts[w][lane][e];
+      }
+      W* row = grad_table + (size_t)key * hidden + column;
+      if constexpr (ADD) add_to_row<W, VEC>(row, load_stream<W, VEC>(row), sum, scale);
+      else write_row<W, VEC>(row, sum, scale);
+    }
+    __syncthreads();
+  }
 }
 
 struct GradientCall {
@@ -413,98 +511,117 @@ struct GradientCall {
 
 inline size_t round_up(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// Sorts the call's tokens; `keys` and `order` receive them.  `spare_*`: as much again, for the passes between.
+template <typename Id, int R>
+int launch_cluster_sort(const GradientCall& call, unsigned ctas, int passes, int digit_bits, const SortedList& list, uint8_t* named, cudaStream_t stream) {
+  if (int status = check_runtime(cudaFuncSetAttribute(sort_in_cluster<Id, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ClusterSort<R>)),
+                                 "cudaFuncSetAttribute(embedding_backward sort)"))
+    return status;
+  launch_dependent_cluster(sort_in_cluster<Id, R>, dim3(ctas), dim3(kSortThreads), ctas, sizeof(ClusterSort<R>), stream,
+                           static_cast<const Id*>(call.tokens), (uint32_t)call.count, (uint32_t)call.vocabulary, call.padding, passes, digit_bits,
+                           (uint32_t)ctas, list, named, device_status_word());
+  return check_launch("embedding_backward sort launch");
+}
+
+// Sorts the call's tokens into `list`.  `spare`: as much again, for the passes between, and `counts`, where there are more
+// than one cluster holds.
 template <typename Id>
-int sort_tokens(const GradientCall& call, uint32_t* keys, uint32_t* order, uint32_t* spare_keys, uint32_t* spare_order, uint32_t* counts,
-                uint8_t* named, cudaStream_t stream) {
+int sort_tokens(const GradientCall& call, const SortedList& list, const SortedList& spare, uint32_t* counts, uint8_t* named, cudaStream_t stream) {
   const uint32_t count = (uint32_t)call.count, vocabulary = (uint32_t)call.vocabulary;
   int bits = 1;  // of the keys 0 .. vocabulary
   while (((unsigned long long)call.vocabulary >> bits) != 0) ++bits;
   const int passes = (bits + kDigitBits - 1) / kDigitBits, digit_bits = (bits + passes - 1) / passes;
+  if (count <= 1024) return launch_cluster_sort<Id, 1>(call, 1, passes, digit_bits, list, named, stream);
+  if (count <= 4096) return launch_cluster_sort<Id, 4>(call, 1, passes, digit_bits, list, named, stream);
+  if (count <= 8192) return launch_cluster_sort<Id, 4>(call, 2, passes, digit_bits, list, named, stream);
+  if (count <= 16384) return launch_cluster_sort<Id, 4>(call, 4, passes, digit_bits, list, named, stream);
+  if (count <= 32768) return launch_cluster_sort<Id, 4>(call, 8, passes, digit_bits, list, named, stream);
+  if (count <= 65536) return launch_cluster_sort<Id, 8>(call, 8, passes, digit_bits, list, named, stream);
   const Id* tokens = static_cast<const Id*>(call.tokens);
-  if (call.count <= (size_t)kTile) {
-    constexpr int kSmem = (2 * kTile + (kSortWarps + 2) * kBins) * (int)sizeof(uint32_t);
-    if (int status = check_runtime(cudaFuncSetAttribute(sort_tokens_small<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem),
-                                   "cudaFuncSetAttribute(embedding_backward sort)"))
-      return status;
-    launch_dependent(sort_tokens_small<Id>, dim3(1), dim3(kSortThreads), kSmem, stream, tokens, count, vocabulary, call.padding, passes,
-                     digit_bits, keys, order, named, device_status_word());
-    return check_launch("embedding_backward sort launch");
-  }
   const int tiles = (int)((call.count + kTile - 1) / kTile);
   const uint32_t mask = (1u << digit_bits) - 1;
-  // the last pass writes `keys` and `order`: with an even number of passes the first one writes the spare pair
+  // the last pass writes `list`: with an even number of passes the first one writes the spare one
   for (int pass = 0; pass < passes; ++pass) {
-    const bool to_result = (passes - 1 - pass) % 2 == 0;
-    uint32_t *keys_to = to_result ? keys : spare_keys, *order_to = to_result ? order : spare_order;
-    const uint32_t *keys_from = to_result ? spare_keys : keys, *order_from = to_result ? spare_order : order;
-    const int shift = pass * digit_bits;
+    const bool to_list = (passes - 1 - pass) % 2 == 0;
+    const SortedList &to = to_list ? list : spare, &from = to_list ? spare : list;
+    const uint32_t *keys_from = from.keys, *order_from = from.order;
+    const int shift = pass * digit_bits, last = pass + 1 == passes;
     if (pass == 0) {
       launch_dependent(count_digits<Id, true>, dim3(tiles), dim3(kSortThreads), 0, stream, tokens, keys_from, count, vocabulary, call.padding,
                        shift, mask, counts, named, device_status_word());
       if (int status = check_launch("embedding_backward count launch")) return status;
       launch_dependent(scatter_digits<Id, true>, dim3(tiles), dim3(kSortThreads), 0, stream, tokens, keys_from, order_from, count, vocabulary,
-                       call.padding, shift, mask, static_cast<const uint32_t*>(counts), tiles, keys_to, order_to);
+                       call.padding, shift, mask, static_cast<const uint32_t*>(counts), tiles, to, last);
     } else {
       launch_dependent(count_digits<Id, false>, dim3(tiles), dim3(kSortThreads), 0, stream, tokens, keys_from, count, vocabulary, call.padding,
                        shift, mask, counts, static_cast<uint8_t*>(nullptr), static_cast<int*>(nullptr));
       if (int status = check_launch("embedding_backward count launch")) return status;
       launch_dependent(scatter_digits<Id, false>, dim3(tiles), dim3(kSortThreads), 0, stream, tokens, keys_from, order_from, count, vocabulary,
-                       call.padding, shift, mask, static_cast<const uint32_t*>(counts), tiles, keys_to, order_to);
+                       call.padding, shift, mask, static_cast<const uint32_t*>(counts), tiles, to, last);
     }
     if (int status = check_launch("embedding_backward scatter launch")) return status;
   }
   return BB200_OK;
 }
 
-template <typename G, typename W, int VEC> int gradient(const GradientCall& call, bool wide_tokens, cudaStream_t stream) {
+template <typename G, typename W, int VEC, bool ADD> int gradient(const GradientCall& call, bool wide_tokens, cudaStream_t stream) {
   const size_t count = call.count, steps = call.hidden / VEC;
-  const size_t tiles = (count + kTile - 1) / kTile;
-  const uint32_t chunk_length = count <= (1u << 16) ? 32 : count <= (1u << 19) ? 128 : 512;
-  const size_t chunks = (count + chunk_length - 1) / chunk_length;
-  const size_t list = round_up(count * 4), counts_bytes = round_up(tiles * kBins * 4), partial = round_up(chunks * 2 * call.hidden * 4);
-  const size_t named_bytes = call.accumulate ? 0 : round_up(call.vocabulary);
+  Segments s = {};
+  s.count = (uint32_t)count;
+  s.vocabulary = (uint32_t)call.vocabulary;
+  s.steps = (int)steps;
+  s.lane_bits = 2;
+  while (s.lane_bits < 8 && ((size_t)1 << s.lane_bits) < steps) ++s.lane_bits;
+  const size_t groups = kThreads >> s.lane_bits, columns = (steps + ((size_t)1 << s.lane_bits) - 1) >> s.lane_bits;
+  // short chunks while there are few tokens, so that the SMs have groups to run; four waves of groups otherwise, at least
+  // eight (one batch) and at most 512 tokens long
+  const size_t resident = ((size_t)multiprocessor_count() * 1024) >> s.lane_bits;
+  s.chunk_length = 8;
+  while (s.chunk_length < 512 && count * columns > (size_t)s.chunk_length * resident * 4) s.chunk_length *= 2;
+  s.chunks = (uint32_t)((count + s.chunk_length - 1) / s.chunk_length);
+  const bool spare = count > 65536;
+  const size_t list = round_up((count + kListTail) * 4), crossings = round_up((1 + (size_t)s.chunks) * 4);
+  const size_t counts_bytes = spare ? round_up((count + kTile - 1) / kTile * kBins * 4) : 0, partial = round_up((size_t)s.chunks * 2 * call.hidden * 4);
+  const size_t named_bytes = ADD ? 0 : round_up(call.vocabulary);
   Workspace workspace(stream);
-  if (int status = workspace.take(4 * list + counts_bytes + partial + named_bytes, "embedding_backward workspace")) return status;
+  if (int status = workspace.take((spare ? 4 : 2) * list + crossings + counts_bytes + partial + named_bytes, "embedding_backward workspace")) return status;
   char* at = workspace.data();
-  uint32_t* lists[4];
-  for (uint32_t*& one : lists) {
-    one = reinterpret_cast<uint32_t*>(at);
-    at += list;
+  const auto next = [&at](size_t bytes) {
+    char* here = at;
+    at += bytes;
+    return here;
+  };
+  SortedList sorted = {}, other = {};
+  sorted.keys = reinterpret_cast<uint32_t*>(next(list));
+  sorted.order = reinterpret_cast<uint32_t*>(next(list));
+  sorted.crossings = other.crossings = reinterpret_cast<uint32_t*>(next(crossings));
+  if (spare) {
+    other.keys = reinterpret_cast<uint32_t*>(next(list));
+    other.order = reinterpret_cast<uint32_t*>(next(list));
   }
-  uint32_t* counts = reinterpret_cast<uint32_t*>(at);
-  float* partials = reinterpret_cast<float*>(at + counts_bytes);
-  uint8_t* named = call.accumulate ? nullptr : reinterpret_cast<uint8_t*>(at + counts_bytes + partial);
+  uint32_t* counts = reinterpret_cast<uint32_t*>(next(counts_bytes));
+  s.partial = reinterpret_cast<float*>(next(partial));
+  uint8_t* named = ADD ? nullptr : reinterpret_cast<uint8_t*>(next(named_bytes));
   if (named) {
     if (int status = check_runtime(cudaMemsetAsync(named, 0, call.vocabulary, stream), "cudaMemsetAsync(embedding_backward)")) return status;
   }
-  if (int status = wide_tokens ? sort_tokens<int64_t>(call, lists[0], lists[1], lists[2], lists[3], counts, named, stream)
-                               : sort_tokens<int32_t>(call, lists[0], lists[1], lists[2], lists[3], counts, named, stream))
+  if (int status = wide_tokens ? sort_tokens<int64_t>(call, sorted, other, counts, named, stream)
+                               : sort_tokens<int32_t>(call, sorted, other, counts, named, stream))
     return status;
-  Segments s = {};
-  s.keys = lists[0];
-  s.order = lists[1];
-  s.partial = partials;
-  s.count = (uint32_t)count;
-  s.vocabulary = (uint32_t)call.vocabulary;
-  s.chunk_length = chunk_length;
-  s.chunks = (uint32_t)chunks;
-  s.steps = (int)steps;
-  s.lane_bits = 5;
-  while (s.lane_bits < 8 && ((size_t)1 << s.lane_bits) < steps) ++s.lane_bits;
-  const size_t groups = kThreads >> s.lane_bits, columns = (steps + ((size_t)1 << s.lane_bits) - 1) >> s.lane_bits;
-  const dim3 grid((unsigned)((chunks + groups - 1) / groups), (unsigned)(columns < 65535 ? columns : 65535));
+  s.keys = sorted.keys;
+  s.order = sorted.order;
+  s.crossings = sorted.crossings;
   W* table = static_cast<W*>(call.grad_table);
-  launch_dependent(sum_chunks<G, W, VEC>, grid, dim3(kThreads), 0, stream, s, static_cast<const G*>(call.grad_out), table, call.scale, call.accumulate);
+  launch_dependent(sum_chunks<G, W, VEC, ADD>, dim3((unsigned)((s.chunks + groups - 1) / groups), (unsigned)(columns < 65535 ? columns : 65535)),
+                   dim3(kThreads), 0, stream, s, static_cast<const G*>(call.grad_out), table, call.scale);
   if (int status = check_launch("embedding_backward sum launch")) return status;
-  if (chunks > 1) {
-    launch_dependent(join_chunks<W, VEC>, grid, dim3(kThreads), 0, stream, s, table, call.scale, call.accumulate);
+  // at most one run crosses each border between two chunks
+  const size_t most_items = (size_t)(s.chunks - 1) * ((steps + 31) / 32), join_most = (size_t)multiprocessor_count() * 4;
+  const unsigned join_blocks = (unsigned)(most_items < join_most ? most_items : join_most);
+  const unsigned fill_blocks = named ? (unsigned)((call.vocabulary + groups - 1) / groups) : 0;
+  if (join_blocks + fill_blocks > 0) {
+    launch_dependent(join_and_fill<W, VEC, ADD>, dim3(join_blocks + fill_blocks), dim3(kThreads), 0, stream, s, table, call.scale, join_blocks,
+                     static_cast<const uint8_t*>(named));
     if (int status = check_launch("embedding_backward join launch")) return status;
-  }
-  if (named) {
-    launch_dependent(zero_unnamed<W, VEC>, dim3((unsigned)((call.vocabulary + groups - 1) / groups)), dim3(kThreads), 0, stream,
-                     static_cast<const uint8_t*>(named), table, s.vocabulary, s.steps, s.lane_bits);
-    if (int status = check_launch("embedding_backward zero launch")) return status;
   }
   return workspace.release("cudaFreeAsync(embedding_backward workspace)");
 }
@@ -563,7 +680,9 @@ struct GradientRun {
   GradientCall call;
   bool wide_tokens;
   cudaStream_t stream;
-  template <typename G, typename W, int VEC> int run() const { return gradient<G, W, VEC>(call, wide_tokens, stream); }
+  template <typename G, typename W, int VEC> int run() const {
+    return call.accumulate ? gradient<G, W, VEC, true>(call, wide_tokens, stream) : gradient<G, W, VEC, false>(call, wide_tokens, stream);
+  }
 };
 
 }  // namespace

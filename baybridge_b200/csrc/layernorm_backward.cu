@@ -24,7 +24,7 @@ template <typename T> struct Backward {
   float* partial;  // [shares][2][hidden]: grad_weight and grad_bias over some of the rows
   size_t rows;
   int hidden;
-  bool wide;  // weight and the column sums are f32
+  bool wide;  // weight and the column sums are f32 beside 16-bit rows
 };
 
 constexpr int kRowThreads = 512, kMostSmem = 204800;
@@ -325,7 +325,7 @@ extern "C" int bb200_layernorm_backward(bb200_dtype dtype, bb200_dtype weight_dt
   if (clash(written, read)) return fail(BB200_E_INVALID_ARGUMENT, "layernorm_backward: an output shares memory with another tensor");
 #define BB200_BACKWARD(T)                                                                                                       \
   backward<T>({static_cast<const T*>(grad_out), static_cast<const T*>(x), mean, rstd, weight, static_cast<const T*>(grad_resid),  \
-               static_cast<T*>(grad_x), nullptr, rows, (int)hidden, weight_dtype == BB200_F32},                                 \
+               static_cast<T*>(grad_x), nullptr, rows, (int)hidden, weight_dtype != dtype},                                 \
               aligned, grad_weight, grad_bias, static_cast<cudaStream_t>(stream))
   switch (dtype) {
     case BB200_BF16: return BB200_BACKWARD(__nv_bfloat16);

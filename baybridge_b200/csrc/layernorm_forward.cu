@@ -4,8 +4,8 @@
 //
 // Bound by HBM bytes: x (and residual) are read once, out (and out_resid) written once.  fp32 throughout, one rounding per
 // output; the variance is the mean of squared differences from the mean, taken from registers, so a large mean costs no
-// precision.  A persistent CTA per SM walks groups of rows (bb200_rows.cuh): weight and bias stay in registers, rows are
-// copied ahead into shared memory, so the two sums of a row wait while the next rows are on their way.
+// precision.  Two forms: many brief CTAs that read the weights again for every row, and persistent CTAs that keep them in
+// registers while rows are copied ahead into shared memory (bb200_rows.cuh); forward() says which is taken when.
 #include "bb200_rows.cuh"
 #include "layernorm_train.h"
 
@@ -24,13 +24,10 @@ template <typename T> struct Forward {
   size_t rows;
   int hidden;
   float epsilon;
-  bool wide;  // weight and bias are f32
+  bool wide;  // weight and bias are f32 beside 16-bit rows
 };
 
-constexpr int kRowThreads = 1024;
-// Shared memory: the rows' slots, then weight and bias as f32, each thread's pairs where it reads them (pair i of lane l at
-// [i / 2][l][i % 2]: 16 bytes a lane, no bank conflict).
-template <typename Rows> constexpr int kVectorBytes = Rows::LANES * Rows::PAIRS * (int)sizeof(F2);
+constexpr int kRowThreads = 512, kMostSmem = 204800;
 
 template <typename T, typename Rows, bool RESIDUAL>
 __global__ void __launch_bounds__(kRowThreads, 1)
@@ -39,26 +36,17 @@ norm_rows(const __grid_constant__ Forward<T> p) {
   extern __shared__ __align__(16) unsigned char shared[];
   __shared__ RowSums<LANES, 1> scratch[GROUPS];
   dependent_launch_prologue();
-  const int group = threadIdx.x / LANES, lane = threadIdx.x % LANES;  // a group's barrier is its own number
+  const int group = threadIdx.x / LANES, lane = threadIdx.x % LANES, barrier = group + 1;
   const T* sources[RESIDUAL ? 2 : 1];
   sources[0] = p.x;
   if constexpr (RESIDUAL) sources[1] = p.residual;
-  Rows rows(shared, sources, p.rows, p.hidden, lane, group, group);
+  Rows rows(shared, sources, p.rows, p.hidden, lane, group, barrier);
   const size_t stride = (size_t)gridDim.x * GROUPS;
   size_t row = (size_t)blockIdx.x * GROUPS + group;
   rows.start(row, stride);
-  F2* weight = reinterpret_cast<F2*>(shared + Rows::kBytes);
-  F2* bias = weight + LANES * PAIRS;
-  if (group == 0) {
-    F2 v[PAIRS];
-    column_pairs<T>(rows, p.weight, p.wide, v);
-#pragma unroll
-    for (int i = 0; i < PAIRS; ++i) weight[((i / 2) * LANES + lane) * 2 + i % 2] = v[i];
-    column_pairs<T>(rows, p.bias, p.wide, v);
-#pragma unroll
-    for (int i = 0; i < PAIRS; ++i) bias[((i / 2) * LANES + lane) * 2 + i % 2] = v[i];
-  }
-  __syncthreads();
+  F2 weight[PAIRS], bias[PAIRS];
+  column_pairs<T>(rows, p.weight, p.wide, weight);
+  column_pairs<T>(rows, p.bias, p.wide, bias);
   const float scale = 1.0f / (float)p.hidden;
   int turn = 0;
   // all groups of the CTA take the same number of turns, so every thread of a warp is there for the exchanges
@@ -81,7 +69,7 @@ norm_rows(const __grid_constant__ Forward<T> p) {
       for (int i = 0; i < PAIRS; ++i) sum2 = sum2 + s[i];
     }
     float sum[1] = {total(sum2)};
-    row_sums<LANES>(sum, &scratch[group], turn, group);
+    row_sums<LANES>(sum, &scratch[group], turn, barrier);
     const float mean = sum[0] * scale;
     F2 centred = both(0.0f);
     if (active) {
@@ -94,7 +82,7 @@ norm_rows(const __grid_constant__ Forward<T> p) {
       }
     }
     sum[0] = total(centred);
-    row_sums<LANES>(sum, &scratch[group], turn, group);
+    row_sums<LANES>(sum, &scratch[group], turn, barrier);
     const float rstd = 1.0f / sqrtf(sum[0] * scale + p.epsilon);
     if (active) {
       if (lane == 0) {
@@ -103,16 +91,105 @@ norm_rows(const __grid_constant__ Forward<T> p) {
       }
       const F2 r = both(rstd);
 #pragma unroll
-      for (int i = 0; i < PAIRS; i += 2) {
-        const int at = ((i / 2) * LANES + lane) * 2;
-        const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(weight + at), b = *reinterpret_cast<const ulonglong2*>(bias + at);
-        s[i] = fma2(s[i] * r, F2{w.x}, F2{b.x});
-        s[i + 1] = fma2(s[i + 1] * r, F2{w.y}, F2{b.y});
-      }
+      for (int i = 0; i < PAIRS; ++i) s[i] = fma2(s[i] * r, weight[i], bias[i]);
       rows.put(p.out + offset, s);
     }
   }
   copy_async_wait<0>();
+}
+
+// Rows of whole vectors with weights of their own type, 16-byte aligned: LANES threads a row, ROWS rows a CTA, no CTA stays.
+// Many small CTAs hide the two sums of a row behind each other's loads.
+template <typename T, int LANES, int ROWS, int VPT, bool RESIDUAL>
+__global__ void __launch_bounds__(LANES * ROWS)
+norm_brief_rows(const __grid_constant__ Forward<T> p) {
+  constexpr int VEC = 16 / sizeof(T), PAIRS = VEC / 2;
+  __shared__ RowSums<LANES, 1> scratch[ROWS];
+  dependent_launch_prologue();
+  const int group = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+  const size_t row = (size_t)blockIdx.x * ROWS + group;
+  if (LANES >= 32 && row >= p.rows) return;
+  const bool active = row < p.rows;
+  const size_t offset = row * (size_t)p.hidden;
+  const float scale = 1.0f / (float)p.hidden;
+  F2 s[VPT][PAIRS];
+  F2 sum2 = both(0.0f);
+  {
+    Pack<T, VEC> a[VPT], b[VPT];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const int c = (lane + j * LANES) * VEC;
+      if (c < p.hidden && active) {
+        a[j] = load_stream<T, VEC>(p.x + offset + c);
+        if constexpr (RESIDUAL) b[j] = load_stream<T, VEC>(p.residual + offset + c);
+      } else {
+        *reinterpret_cast<uint4*>(&a[j]) = make_uint4(0, 0, 0, 0);
+        if constexpr (RESIDUAL) *reinterpret_cast<uint4*>(&b[j]) = make_uint4(0, 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) {
+        s[j][i] = Pairs<T>::get(a[j], i);
+        if constexpr (RESIDUAL) {
+          s[j][i] = s[j][i] + Pairs<T>::get(b[j], i);
+          Pairs<T>::set(a[j], i, s[j][i]);
+        }
+        sum2 = sum2 + s[j][i];
+      }
+      if constexpr (RESIDUAL) {
+        const int c = (lane + j * LANES) * VEC;
+        if (c < p.hidden && active) store_stream<T, VEC>(p.out_resid + offset + c, a[j]);
+      }
+    }
+  }
+  int turn = 0;
+  float sum[1] = {total(sum2)};
+  row_sums<LANES>(sum, &scratch[group], turn, group);
+  const float mean = sum[0] * scale;
+  const F2 minus_mean = both(-mean);
+  F2 centred = both(0.0f);
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    F2 part = both(0.0f);
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+      s[j][i] = s[j][i] + minus_mean;
+      part = fma2(s[j][i], s[j][i], part);
+    }
+    if ((lane + j * LANES) * VEC < p.hidden) centred = centred + part;
+  }
+  sum[0] = total(centred);
+  row_sums<LANES>(sum, &scratch[group], turn, group);
+  const float rstd = 1.0f / sqrtf(sum[0] * scale + p.epsilon);
+  if (!active) return;
+  if (lane == 0) {
+    p.mean[row] = mean;
+    p.rstd[row] = rstd;
+  }
+  const F2 r = both(rstd);
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int c = (lane + j * LANES) * VEC;
+    if (c < p.hidden) {
+      Pack<T, VEC> o;
+      const Pack<T, VEC> w = load_shared_operand<T, VEC>(static_cast<const T*>(p.weight) + c);
+      Pack<T, VEC> b;
+      *reinterpret_cast<uint4*>(&b) = make_uint4(0, 0, 0, 0);
+      if (p.bias) b = load_shared_operand<T, VEC>(static_cast<const T*>(p.bias) + c);
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) Pairs<T>::set(o, i, fma2(s[j][i] * r, Pairs<T>::get(w, i), Pairs<T>::get(b, i)));
+      store_stream<T, VEC>(p.out + offset + c, o);
+    }
+  }
+}
+
+template <typename T, int LANES, int ROWS, int VPT> int launch_brief(const Forward<T>& p, cudaStream_t stream) {
+  const dim3 grid((unsigned)((p.rows + ROWS - 1) / ROWS)), block(LANES * ROWS);
+  if (p.residual) launch_dependent(norm_brief_rows<T, LANES, ROWS, VPT, true>, grid, block, 0, stream, p);
+  else launch_dependent(norm_brief_rows<T, LANES, ROWS, VPT, false>, grid, block, 0, stream, p);
+  return check_launch("layernorm_forward kernel launch");
 }
 
 // One row to a CTA, all of it in registers: rows too long for the kernel above (more than 2048 vectors).
@@ -231,12 +308,11 @@ norm_rows_by_element(const __grid_constant__ Forward<T> p) {
 }
 
 template <typename T, typename Rows, bool RESIDUAL> int launch_rows(const Forward<T>& p, cudaStream_t stream) {
-  constexpr int kSmem = Rows::kBytes + 2 * kVectorBytes<Rows>;
   const auto kernel = norm_rows<T, Rows, RESIDUAL>;
-  if (int status = check_runtime(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem), "cudaFuncSetAttribute(layernorm_forward)"))
+  if (int status = check_runtime(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Rows::kBytes), "cudaFuncSetAttribute(layernorm_forward)"))
     return status;
   const size_t wanted = (p.rows + Rows::GROUPS - 1) / Rows::GROUPS, most = (size_t)multiprocessor_count();
-  launch_dependent(kernel, dim3((unsigned)(wanted < most ? wanted : most)), dim3(kRowThreads), (size_t)kSmem, stream, p);
+  launch_dependent(kernel, dim3((unsigned)(wanted < most ? wanted : most)), dim3(kRowThreads), (size_t)Rows::kBytes, stream, p);
   return check_launch("layernorm_forward kernel launch");
 }
 
@@ -244,19 +320,33 @@ template <typename T> int forward(const Forward<T>& p, bool aligned, cudaStream_
   constexpr int VEC = 16 / sizeof(T);
   const int nvec = p.hidden / VEC;
   if (aligned && p.hidden % VEC == 0) {
-    // two vectors a thread, so that 1024 threads an SM fit the registers; weight and bias take 8 bytes a column of the memory
+    // Weights of the rows' own type are read again for every row (from L1 and L2, 16 bytes a load); f32 weights beside 16-bit
+    // rows would be twice the rows' own bytes, so they stay in a persistent kernel's registers.  65536 rows, bf16: brief
+    // kernel and persistent one with bf16 weights 84 and 97 us (1024 wide, residual), 315 and 352 us (4096, residual), 392 and
+    // 395 us (8192); with f32 weights 176 and 95 us (2048), 833 and 660 us (8192, residual).
+    if (!p.wide && nvec <= 512 && aligned16(p.weight) && aligned16(p.bias)) {
+      if (nvec <= 8) return launch_brief<T, 8, 32, 1>(p, stream);
+      if (nvec <= 16) return launch_brief<T, 16, 16, 1>(p, stream);
+      if (nvec <= 32) return launch_brief<T, 32, 8, 1>(p, stream);
+      if (nvec <= 64) return launch_brief<T, 32, 8, 2>(p, stream);
+      if (nvec <= 128) return launch_brief<T, 32, 8, 4>(p, stream);
+      if (nvec <= 256) return launch_brief<T, 128, 2, 2>(p, stream);
+      return launch_brief<T, 256, 1, 2>(p, stream);
+    }
+    // Up to 32 columns a thread, whose weight and bias fit the registers beside the row; two groups of 256 threads hide each
+    // other's sums (8192 wide, bf16: 395 us against 523 us for one group of 512).
 #define BB200_VECTOR_ROWS(LANES, VPT)                                                              \
   if (nvec <= (LANES) * (VPT))                                                                     \
-    return p.residual ? launch_rows<T, VectorRows<T, kRowThreads, LANES, VPT, 2, 1, 221184 - (LANES) * (VPT) * 16 / (int)sizeof(T) * 8>, true>(p, stream) : launch_rows<T, VectorRows<T, kRowThreads, LANES, VPT, 1, 1, 221184 - (LANES) * (VPT) * 16 / (int)sizeof(T) * 8>, false>(p, stream)
+    return p.residual ? launch_rows<T, VectorRows<T, kRowThreads, LANES, VPT, 2, 1, kMostSmem>, true>(p, stream) : launch_rows<T, VectorRows<T, kRowThreads, LANES, VPT, 1, 1, kMostSmem>, false>(p, stream)
     BB200_VECTOR_ROWS(4, 2);
     BB200_VECTOR_ROWS(8, 2);
     BB200_VECTOR_ROWS(16, 2);
     BB200_VECTOR_ROWS(32, 2);
-    BB200_VECTOR_ROWS(64, 2);
-    BB200_VECTOR_ROWS(128, 2);
+    BB200_VECTOR_ROWS(32, 4);
+    BB200_VECTOR_ROWS(64, 4);
     BB200_VECTOR_ROWS(256, 2);
-    BB200_VECTOR_ROWS(512, 2);
-    if constexpr (VEC == 4) BB200_VECTOR_ROWS(1024, 2);
+    BB200_VECTOR_ROWS(256, 4);
+    if constexpr (VEC == 4) BB200_VECTOR_ROWS(512, 4);
 #undef BB200_VECTOR_ROWS
     if (nvec <= 2048) launch_dependent(norm_long_rows<T, 1024, 2>, dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
     else launch_dependent(norm_long_rows<T, 1024, 4>, dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
@@ -265,8 +355,8 @@ template <typename T> int forward(const Forward<T>& p, bool aligned, cudaStream_
   if (aligned) {
 #define BB200_SHIFTED_ROWS(LANES, COLUMNS, SURE)                                                       \
   if (p.hidden <= (LANES) * (COLUMNS))                                                             \
-    return p.residual ? launch_rows<T, ShiftedRows<T, kRowThreads, LANES, COLUMNS, SURE, 2, 1, 221184 - (LANES) * (COLUMNS) * 8>, true>(p, stream) : launch_rows<T, ShiftedRows<T, kRowThreads, LANES, COLUMNS, SURE, 1, 1, 221184 - (LANES) * (COLUMNS) * 8>, false>(p, stream)
-    constexpr int kColumns = 2 * VEC;
+    return p.residual ? launch_rows<T, ShiftedRows<T, kRowThreads, LANES, COLUMNS, SURE, 2, 1, kMostSmem>, true>(p, stream) : launch_rows<T, ShiftedRows<T, kRowThreads, LANES, COLUMNS, SURE, 1, 1, kMostSmem>, false>(p, stream)
+    constexpr int kColumns = 16;
     BB200_SHIFTED_ROWS(32, 4, 0);
     BB200_SHIFTED_ROWS(32, kColumns / 2, 4);
     BB200_SHIFTED_ROWS(32, kColumns, kColumns / 2);
@@ -274,7 +364,6 @@ template <typename T> int forward(const Forward<T>& p, bool aligned, cudaStream_
     BB200_SHIFTED_ROWS(128, kColumns, kColumns / 2);
     BB200_SHIFTED_ROWS(256, kColumns, kColumns / 2);
     BB200_SHIFTED_ROWS(512, kColumns, kColumns / 2);
-    if constexpr (VEC == 4) BB200_SHIFTED_ROWS(1024, kColumns, kColumns / 2);
 #undef BB200_SHIFTED_ROWS
   }
   const int smem = p.hidden * (int)sizeof(float);
@@ -315,7 +404,7 @@ extern "C" int bb200_layernorm_forward(bb200_dtype dtype, bb200_dtype weight_dty
     return fail(BB200_E_INVALID_ARGUMENT, "layernorm_forward: an output shares memory with another tensor");
 #define BB200_FORWARD(T)                                                                                                          \
   forward<T>({static_cast<const T*>(x), static_cast<const T*>(residual), weight, bias, static_cast<T*>(out), static_cast<T*>(out_resid), \
-              mean, rstd, rows, (int)hidden, epsilon, weight_dtype == BB200_F32},                                                 \
+              mean, rstd, rows, (int)hidden, epsilon, weight_dtype != dtype},                                                 \
              aligned, static_cast<cudaStream_t>(stream))
   switch (dtype) {
     case BB200_BF16: return BB200_FORWARD(__nv_bfloat16);
