@@ -152,15 +152,38 @@ class B200Backend:
             "adamw": self._adamw_runner,
         }[plan.kind](ir, plan, record, state)
         arguments = ir.arguments
-        # what a device tensor handle must look like per argument, computed once
-        expected = [(tuple(a.spec.shape), a.spec.dtype, row_major_stride(a.spec.shape)) if a.kind == "tensor" else None for a in arguments]
-        tensor_positions = [position for position, a in enumerate(arguments) if a.kind == "tensor"]
-        all_tensors = len(tensor_positions) == len(arguments)
+        # what a device tensor handle must look like per argument (``TensorHandle.signature``), computed once
+        signatures = [(a.spec.dtype, tuple(a.spec.shape), DLPACK_CUDA, True) if a.kind == "tensor" else None for a in arguments]
         # kernels that can record a code in the device status word: the mbarrier pipelines (bounded waits), the
         # bounds-checking debug build of thread-by-thread elementwise kernels, and the lookups (tokens outside the table)
         waits_on_device = plan.kind in ("gemm", "attention", "embedding", "embedding_backward") or bool(record.get("debug_bounds"))
-        checked: dict[tuple[int, int], Any] = {}  # (argument position, id of handle) -> handle already validated there
 
+        def quick(values: Any, stream: Any) -> bool:
+            """The hot call: launches and returns True when every argument is a dense CUDA tensor handle of the expected
+            shape and dtype, all on one device, and nothing has to be waited for; False sends the caller to the general
+            path, which also produces the error messages."""
+            if self.synchronize and not native.recording():
+                return False
+            pointers = []
+            device_id = None
+            for value, signature in zip(values, signatures):
+                if type(value) is not TensorHandle or value.signature != signature:
+                    return False
+                if device_id is None:
+                    device_id = value.device_id
+                elif value.device_id != device_id:
+                    return False
+                pointer = value.raw_address or value.data_ptr()
+                if not pointer:
+                    return False
+                pointers.append(pointer)
+            native.require_device()
+            _bind_device(device_id)
+            runner(pointers, {}, None if stream is None else native.stream_handle(stream))
+            LAUNCH_COUNTER["launches"] += 1
+            return True
+
+        all_tensors = bool(arguments) and all(a.kind == "tensor" for a in arguments)
         def launcher(*args: Any, **kwargs: Any) -> None:
             stream = kwargs.pop("stream", None)
             if kwargs:
@@ -169,35 +192,8 @@ class B200Backend:
                 raise TypeError(f"{ir.name} expects {len(arguments)} arguments, got {len(args)}")
             native.require_device()
             synchronize = self.synchronize and not native.recording()  # a recording stream must not be synchronised
-            if all_tensors and not synchronize:
-                # fast path: every argument is a contiguous CUDA tensor handle of the expected shape and dtype on one
-                # device; anything else takes the general path below, which also produces the error messages
-                pointers = {}
-                device_id = None
-                for position in tensor_positions:
-                    value = args[position]
-                    known = checked.get((position, id(value)))
-                    if known is not value:
-                        # a handle is immutable: its shape, dtype and strides are compared once per argument position
-                        shape, dtype, stride = expected[position]
-                        if (type(value) is not TensorHandle or value.device_type != DLPACK_CUDA or tuple(value.shape) != shape
-                                or normalize_dtype_name(value.dtype) != dtype or (value.stride is not None and tuple(value.stride) != stride)):
-                            break
-                        if len(checked) >= 256:
-                            checked.clear()
-                        checked[(position, id(value))] = value  # keeps the handle alive, so its id cannot be reused
-                    if device_id is not None and value.device_id != device_id:
-                        break
-                    device_id = value.device_id
-                    pointer = value.data_ptr() or value.raw_address
-                    if not pointer:
-                        break
-                    pointers[position] = int(pointer)
-                else:
-                    _bind_device(int(device_id))
-                    runner(pointers, {}, native.stream_handle(stream))
-                    LAUNCH_COUNTER["launches"] += 1
-                    return
+            if all_tensors and quick(args, stream):
+                return
             staged: list[tuple[RuntimeTensor, _StagedSlot, Any]] = []
             stream_handle = native.stream_handle(stream)
             try:
@@ -247,6 +243,8 @@ class B200Backend:
                     native.library().bb200_module_unload(module)
                 holder.get("functions", {}).clear()
 
+        if all_tensors:
+            launcher.quick = quick  # type: ignore[attr-defined]
         if isinstance(plan, AdamWPlan):
             launcher.grouped = self._adamw_grouped(ir, plan, state)  # type: ignore[attr-defined]
         launcher.plan = plan  # type: ignore[attr-defined]
@@ -539,21 +537,24 @@ class B200Backend:
     def _embedding_runner(self, ir, plan: EmbeddingPlan, record, state):
         entry, codes = native.entry_point("bb200_embedding"), native.DTYPE_CODES
         dtypes = codes[plan.table_dtype], codes[plan.out_dtype], codes[plan.token_dtype]
+        extents = plan.count, plan.vocabulary, plan.hidden, plan.scale
 
         def run(pointers, scalars, stream_handle) -> None:
-            native.call_resolved(entry, "bb200_embedding", *dtypes, pointers[plan.tokens], pointers[plan.table], pointers[plan.out],
-                                 plan.count, plan.vocabulary, plan.hidden, plan.scale, stream_handle)
+            status = entry(*dtypes, pointers[plan.tokens], pointers[plan.table], pointers[plan.out], *extents, stream_handle)
+            if status:
+                native.raise_status("bb200_embedding", status)
 
         return run
 
     def _embedding_backward_runner(self, ir, plan: EmbeddingBackwardPlan, record, state):
         entry, codes = native.entry_point("bb200_embedding_backward"), native.DTYPE_CODES
         dtypes = codes[plan.grad_dtype], codes[plan.table_dtype], codes[plan.token_dtype]
+        extents = plan.count, plan.vocabulary, plan.hidden, plan.scale, plan.padding_token, int(plan.accumulate)
 
         def run(pointers, scalars, stream_handle) -> None:
-            native.call_resolved(entry, "bb200_embedding_backward", *dtypes, pointers[plan.grad_out], pointers[plan.tokens],
-                                 pointers[plan.grad_table], plan.count, plan.vocabulary, plan.hidden, plan.scale, plan.padding_token,
-                                 int(plan.accumulate), stream_handle)
+            status = entry(*dtypes, pointers[plan.grad_out], pointers[plan.tokens], pointers[plan.grad_table], *extents, stream_handle)
+            if status:
+                native.raise_status("bb200_embedding_backward", status)
 
         return run
 
@@ -561,11 +562,12 @@ class B200Backend:
         entry, codes = native.entry_point("bb200_layernorm_forward"), native.DTYPE_CODES
         dtypes = codes[plan.dtype], codes[plan.weight_dtype]
         order = (plan.x, plan.residual, plan.weight, plan.bias, plan.out, plan.out_resid, plan.mean, plan.rstd)
+        extents = plan.rows, plan.hidden, plan.epsilon
 
         def run(pointers, scalars, stream_handle) -> None:
-            native.call_resolved(entry, "bb200_layernorm_forward", *dtypes,
-                                 *[None if position is None else pointers[position] for position in order],
-                                 plan.rows, plan.hidden, plan.epsilon, stream_handle)
+            status = entry(*dtypes, *[None if position is None else pointers[position] for position in order], *extents, stream_handle)
+            if status:
+                native.raise_status("bb200_layernorm_forward", status)
 
         return run
 
@@ -573,11 +575,12 @@ class B200Backend:
         entry, codes = native.entry_point("bb200_layernorm_backward"), native.DTYPE_CODES
         dtypes = codes[plan.dtype], codes[plan.weight_dtype]
         order = (plan.grad_out, plan.x, plan.mean, plan.rstd, plan.weight, plan.grad_resid, plan.grad_x, plan.grad_weight, plan.grad_bias)
+        rows, hidden = plan.rows, plan.hidden
 
         def run(pointers, scalars, stream_handle) -> None:
-            native.call_resolved(entry, "bb200_layernorm_backward", *dtypes,
-                                 *[None if position is None else pointers[position] for position in order],
-                                 plan.rows, plan.hidden, stream_handle)
+            status = entry(*dtypes, *[None if position is None else pointers[position] for position in order], rows, hidden, stream_handle)
+            if status:
+                native.raise_status("bb200_layernorm_backward", status)
 
         return run
 
@@ -589,10 +592,12 @@ class B200Backend:
         param_dtypes = (ctypes.c_int * count)(*(native.DTYPE_CODES[name] for name in plan.param_dtypes))
         grad_dtypes = (ctypes.c_int * count)(*(native.DTYPE_CODES[name] for name in plan.grad_dtypes))
         decays = (ctypes.c_float * count)(*plan.weight_decay)
+        beta1, beta2, epsilon = plan.beta1, plan.beta2, plan.epsilon
 
         def step(lists, schedule, stream_handle) -> None:
-            native.call_resolved(entry, "bb200_adamw", count, numels, param_dtypes, grad_dtypes, decays, *lists, schedule,
-                                 plan.beta1, plan.beta2, plan.epsilon, stream_handle)
+            status = entry(count, numels, param_dtypes, grad_dtypes, decays, *lists, schedule, beta1, beta2, epsilon, stream_handle)
+            if status:
+                native.raise_status("bb200_adamw", status)
 
         return step
 
@@ -615,24 +620,24 @@ class B200Backend:
         contiguous = all(role == tuple(range(role[0], role[0] + count)) for role in roles)
         expected = [group_signature((ir.arguments[p].spec.dtype, ir.arguments[p].spec.shape) for p in role) for role in roles]
         names = ("params", "grads", "exp_avgs", "exp_avg_sqs", "masters")
+        firsts, schedule_signature = [role[0] for role in roles], ("f32", (3,), DLPACK_CUDA, True)
 
         def grouped(values: dict[int, Any], stream: Any) -> bool:
             schedule = values.get(plan.schedule)
-            if not contiguous or type(schedule) is not TensorHandle or len(values) != len(roles) + 1:
+            if not contiguous or type(schedule) is not TensorHandle or schedule.signature != schedule_signature or len(values) != len(roles) + 1:
                 return False
-            groups = [values.get(role[0]) for role in roles]
-            if any(type(group) is not TensorGroup for group in groups):
-                return False
+            groups = [values.get(first) for first in firsts]
+            for group in groups:
+                if type(group) is not TensorGroup:
+                    return False
             for name, group, signature in zip(names, groups, expected):
                 if group.signature != signature:
                     raise TypeError(f"b200: the {name} of {ir.name} differ in number, dtype or shape from those it was compiled for")
                 if group.device_id != schedule.device_id:
                     raise BackendNotImplementedError("b200: tensor arguments live on different devices")
-            if schedule.device_type != DLPACK_CUDA or schedule.shape != (3,) or schedule.dtype != "f32" or not schedule.is_contiguous:
-                raise TypeError(f"b200 tensor argument '{ir.arguments[plan.schedule].name}' expects a dense CUDA f32 tensor of shape (3,)")
             native.require_device()
             _bind_device(int(schedule.device_id))
-            stream_handle = native.stream_handle(stream)
+            stream_handle = None if stream is None else native.stream_handle(stream)
             lists = [group.addresses for group in groups]
             step(lists if plan.masters else lists + [None], schedule.data_ptr(), stream_handle)
             LAUNCH_COUNTER["launches"] += 1

@@ -203,13 +203,17 @@ def library() -> ctypes.CDLL:
     return lib
 
 
+def raise_status(name: str, status: int) -> None:
+    """Raise what a non-zero status of the entry point ``name`` means."""
+    message = (library().bb200_last_error() or b"").decode("utf-8", "replace")
+    raise CudaDriverError(name, status, ERROR_NAMES.get(status, "CUDA_ERROR" if status > 0 else "BB200_ERROR"), message)
+
+
 def call(name: str, *args: Any) -> None:
     """Invoke ``lib.<name>(*args)`` and raise ``CudaDriverError`` on a non-zero status."""
-    lib = library()
-    status = getattr(lib, name)(*args)
+    status = getattr(library(), name)(*args)
     if status != 0:
-        message = (lib.bb200_last_error() or b"").decode("utf-8", "replace")
-        raise CudaDriverError(name, status, ERROR_NAMES.get(status, "CUDA_ERROR" if status > 0 else "BB200_ERROR"), message)
+        raise_status(name, status)
 
 
 def entry_point(name: str) -> Any:
@@ -221,8 +225,7 @@ def call_resolved(function: Any, name: str, *args: Any) -> None:
     """``call`` for a function obtained from ``entry_point``."""
     status = function(*args)
     if status != 0:
-        message = (library().bb200_last_error() or b"").decode("utf-8", "replace")
-        raise CudaDriverError(name, status, ERROR_NAMES.get(status, "CUDA_ERROR" if status > 0 else "BB200_ERROR"), message)
+        raise_status(name, status)
 
 
 def take_device_status(stream: ctypes.c_void_p) -> int:

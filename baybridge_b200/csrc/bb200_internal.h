@@ -4,6 +4,8 @@
 #include <stdarg.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/bb200.h"
 
 namespace bb200 {
@@ -114,6 +116,19 @@ class Workspace {
   cudaStream_t stream_;
   char* data_ = nullptr;
 };
+
+// Raise KERNEL's limit of dynamic shared memory to `bytes` on the current device, once per kernel and device (`bytes` is the
+// same in every call; two threads doing it at once is harmless).
+template <auto KERNEL> int allow_shared_memory(int bytes, const char* what) {
+  static std::atomic<bool> done[kMaxWorkspaceDevices];
+  int device = 0;
+  if (int status = check_runtime(cudaGetDevice(&device), what)) return status;
+  const bool known = device >= 0 && device < kMaxWorkspaceDevices;
+  if (known && done[device].load(std::memory_order_relaxed)) return BB200_OK;
+  if (int status = check_runtime(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what)) return status;
+  if (known) done[device].store(true, std::memory_order_relaxed);
+  return BB200_OK;
+}
 
 // Whether [a, a + a_bytes) and [b, b + b_bytes) share memory (null pointers share none).
 inline bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {

@@ -18,19 +18,50 @@
 //
 // Tokens outside [0, vocabulary) read as zeros (lookup) or contribute nothing (gradient) and are recorded in the device
 // status word.  A padding token and out-of-range tokens sort behind every row under the key `vocabulary`.
-#include "bb200_elementwise.cuh"
 #include "bb200_internal.h"
+#include "bb200_rows.cuh"
 
 namespace bb200 {
 namespace {
 
 constexpr int kThreads = 256;
 
-// The row vectors of one step: VEC elements, widened.
-template <typename T, int VEC> __device__ __forceinline__ void widen(const Pack<T, VEC>& in, float (&out)[VEC]) {
+// The fp32 sum of some rows' vectors: VEC elements, in pairs where there are any.
+template <int VEC> struct Sum {
+  F2 pair[VEC / 2];
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) out[e] = Conv<float, T>::widen(in.v[e]);
-}
+    for (int i = 0; i < VEC / 2; ++i) pair[i] = both(0.0f);
+  }
+  template <typename T> __device__ __forceinline__ void add(const Pack<T, VEC>& v) {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) pair[i] = pair[i] + Pairs<T>::get(v, i);
+  }
+  // the sum times `scale` (and plus `old`), rounded once
+  template <typename T> __device__ __forceinline__ Pack<T, VEC> times(float scale) const {
+    Pack<T, VEC> r;
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) Pairs<T>::set(r, i, pair[i] * both(scale));
+    return r;
+  }
+  template <typename T> __device__ __forceinline__ Pack<T, VEC> times_plus(float scale, const Pack<T, VEC>& old) const {
+    Pack<T, VEC> r;
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) Pairs<T>::set(r, i, fma2(pair[i], both(scale), Pairs<T>::get(old, i)));
+    return r;
+  }
+  __device__ __forceinline__ Pack<float, VEC> values() const { return times<float>(1.0f); }
+};
+template <> struct Sum<1> {
+  float value;
+  __device__ __forceinline__ void clear() { value = 0.0f; }
+  template <typename T> __device__ __forceinline__ void add(const Pack<T, 1>& v) { value += Conv<float, T>::widen(v.v[0]); }
+  template <typename T> __device__ __forceinline__ Pack<T, 1> times(float scale) const { return {{Conv<float, T>::narrow(value * scale)}}; }
+  template <typename T> __device__ __forceinline__ Pack<T, 1> times_plus(float scale, const Pack<T, 1>& old) const {
+    return {{Conv<float, T>::narrow(fmaf(value, scale, Conv<float, T>::widen(old.v[0])))}};
+  }
+  __device__ __forceinline__ Pack<float, 1> values() const { return {{value}}; }
+};
 
 // ---- lookup -------------------------------------------------------------------------------------------------------
 // `1 << lane_bits` neighbouring threads share a row; each moves two vectors of it per pass over the columns, so 2048
@@ -83,7 +114,7 @@ int launch_lookup(const void* tokens, const void* table, void* out, size_t count
 // ---- sorting the tokens ---------------------------------------------------------------------------------------------
 // Least-significant-digit radix sort of (token, position), stable, digits of at most 9 bits.  A CTA ranks 1024 * R elements:
 // warp w holds elements [32 R w, 32 R (w + 1)), 32 at a time in order; within 32 the rank among equal digits comes from
-// __match_any_sync, earlier 32s of the warp are counted in the warp's own shared-memory counters, and earlier warps by a
+// a ballot per bit, earlier 32s of the warp are counted in the warp's own shared-memory counters, and earlier warps by a
 // prefix over the 32 counters of a digit.
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kDigitBits = 9, kBins = 1 << kDigitBits;
 // 16-bit counters, two digits to a word; rows of 257 words keep the prefix over warps free of bank conflicts.
@@ -100,14 +131,19 @@ template <typename Id> __device__ __forceinline__ uint32_t key_of(Id raw, uint32
 
 // Stable rank of each of a thread's R elements among the CTA's elements of the same digit; totals[d] = how many there are.
 template <int R>
-__device__ __forceinline__ void rank_digits(const uint32_t (&digit)[R], uint32_t (&rank)[R], uint32_t (*counters)[kCounterWords], uint32_t* totals) {
+__device__ __forceinline__ void rank_digits(const uint32_t (&digit)[R], uint32_t (&rank)[R], int digit_bits, uint32_t (*counters)[kCounterWords], uint32_t* totals) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int word = lane; word < kCounterWords; word += 32) counters[warp][word] = 0;
   uint16_t* mine = reinterpret_cast<uint16_t*>(counters[warp]);
   __syncwarp();
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const uint32_t same = __match_any_sync(0xffffffffu, digit[r]);
+    uint32_t same = 0xffffffffu;
+    for (int bit = 0; bit < digit_bits; ++bit) {
+      const bool set = (digit[r] >> bit) & 1;
+      const uint32_t vote = __ballot_sync(0xffffffffu, set);
+      same &= set ? vote : ~vote;
+    }
     const uint32_t before = __popc(same & ((1u << lane) - 1));
     rank[r] = mine[digit[r]] + before;
     __syncwarp();
@@ -164,19 +200,11 @@ __device__ __forceinline__ uint32_t exclusive_over_bins(uint32_t value, uint32_t
   return others + inclusive - value;
 }
 
-// Behind the sorted list stand a few keys that no row has, so that readers may look ahead of its end.
-constexpr int kListTail = 16;
-
 struct SortedList {
   uint32_t* keys;
   uint32_t* order;
   uint32_t* crossings;  // [0]: how many runs cross a chunk's border (set to 0 here), then their first chunks
 };
-
-__device__ __forceinline__ void finish_list(const SortedList& list, uint32_t count, uint32_t vocabulary) {
-  if (blockIdx.x == 0 && threadIdx.x < kListTail) list.keys[count + threadIdx.x] = vocabulary;
-  if (blockIdx.x == 0 && threadIdx.x == kListTail) list.crossings[0] = 0;
-}
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -194,8 +222,8 @@ __device__ __forceinline__ uint32_t in_cta(const void* shared, uint32_t rank) {
 }
 
 // Up to 65536 tokens in one launch: one cluster of 1, 2, 4 or 8 CTAs holds them all in shared memory.  Every pass ranks in
-// each CTA, adds up the CTAs' digit counts through distributed shared memory and sends every element to its place, the
-// last pass to global memory.
+// each CTA, adds up the CTAs' digit counts through distributed shared memory and sends every element to its place there;
+// nobody touches another CTA's memory after the last pass's barrier.
 template <int R> struct ClusterSort {
   uint2 pairs[kSortThreads * R];
   uint32_t counters[kSortWarps][kCounterWords];
@@ -222,12 +250,12 @@ sort_in_cluster(const Id* __restrict__ tokens, uint32_t count, uint32_t vocabula
     key[r] = position[r] < count ? key_of(tokens[position[r]], vocabulary, padding, status_word) : vocabulary;
     if (named && key[r] < vocabulary) named[key[r]] = 1;
   }
-  finish_list(list, count, vocabulary);
+  if (blockIdx.x == 0 && threadIdx.x == 0) list.crossings[0] = 0;
   for (int pass = 0; pass < passes; ++pass) {
     uint32_t digit[R], rank[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) digit[r] = (key[r] >> (pass * digit_bits)) & ((1u << digit_bits) - 1);
-    rank_digits<R>(digit, rank, s.counters, s.totals);
+    rank_digits<R>(digit, rank, digit_bits, s.counters, s.totals);
     uint32_t total = 0, earlier = 0;
     if (ctas > 1) cluster_barrier();  // every CTA's totals stand
     if (threadIdx.x < kBins) {
@@ -241,32 +269,28 @@ sort_in_cluster(const Id* __restrict__ tokens, uint32_t count, uint32_t vocabula
     const uint32_t start = exclusive_over_bins(total, s.warp_totals) + earlier;
     if (threadIdx.x < kBins) s.starts[threadIdx.x] = start;
     __syncthreads();
-    if (pass + 1 < passes) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const uint32_t to = s.starts[digit[r]] + rank[r];
-        asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(in_cta(&s.pairs[to % kEach], to / kEach)), "r"(key[r]), "r"(position[r]) : "memory");
-      }
-      if (ctas > 1) cluster_barrier();  // everything has arrived, and every CTA has read the totals
-      else __syncthreads();
+    for (int r = 0; r < R; ++r) {
+      const uint32_t to = s.starts[digit[r]] + rank[r];
+      asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(in_cta(&s.pairs[to % kEach], to / kEach)), "r"(key[r]), "r"(position[r]) : "memory");
+    }
+    if (ctas > 1) cluster_barrier();  // everything has arrived, and every CTA has read the totals
+    else __syncthreads();
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const uint2 pair = s.pairs[warp * (32 * R) + r * 32 + lane];
-        key[r] = pair.x;
-        position[r] = pair.y;
-      }
-    } else {
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const uint32_t to = s.starts[digit[r]] + rank[r];
-        if (to < count) {
-          list.keys[to] = key[r];
-          list.order[to] = position[r];
-        }
-      }
+    for (int r = 0; r < R; ++r) {
+      const uint2 pair = s.pairs[warp * (32 * R) + r * 32 + lane];
+      key[r] = pair.x;
+      position[r] = pair.y;
     }
   }
-  if (ctas > 1) cluster_barrier();  // nobody leaves while another CTA still reads its totals
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const uint32_t at = rank_of_cta * kEach + warp * (32 * R) + r * 32 + lane;
+    if (at < count) {
+      list.keys[at] = key[r];
+      list.order[at] = position[r];
+    }
+  }
 }
 
 // More tokens: per digit a launch that counts and a launch that scatters, a tile of 8192 to a CTA.
@@ -338,7 +362,7 @@ scatter_digits(const Id* __restrict__ tokens, const uint32_t* __restrict__ keys,
     }
     digit[r] = valid ? (key[r] >> shift) & mask : kBins - 1;
   }
-  rank_digits<kTileRounds>(digit, rank, counters, totals);
+  rank_digits<kTileRounds>(digit, rank, kDigitBits, counters, totals);
 #pragma unroll
   for (int r = 0; r < kTileRounds; ++r) {
     const size_t at = (size_t)blockIdx.x * kTile + warp * (32 * kTileRounds) + r * 32 + lane;
@@ -348,30 +372,12 @@ scatter_digits(const Id* __restrict__ tokens, const uint32_t* __restrict__ keys,
       list.order[to] = position[r];
     }
   }
-  if (last) finish_list(list, count, vocabulary);
+  if (last && blockIdx.x == 0 && threadIdx.x == 0) list.crossings[0] = 0;
 }
 
 // ---- segmented sums ---------------------------------------------------------------------------------------------------
-template <typename W, int VEC> __device__ __forceinline__ void write_row(W* __restrict__ row, const float (&sum)[VEC], float scale) {
-  Pack<W, VEC> r;
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) r.v[e] = Conv<float, W>::narrow(sum[e] * scale);
-  store_stream<W, VEC>(row, r);
-}
-template <typename W, int VEC>
-__device__ __forceinline__ void add_to_row(W* __restrict__ row, const Pack<W, VEC>& old, const float (&sum)[VEC], float scale) {
-  Pack<W, VEC> r;
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) r.v[e] = Conv<float, W>::narrow(fmaf(sum[e], scale, Conv<float, W>::widen(old.v[e])));
-  store_stream<W, VEC>(row, r);
-}
-template <int VEC> __device__ __forceinline__ void keep_partial(float* to, const float (&sum)[VEC]) {
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) to[e] = sum[e];
-}
-
 struct Segments {
-  const uint32_t* keys;   // sorted tokens, with a tail of keys that no row has
+  const uint32_t* keys;   // sorted tokens
   const uint32_t* order;  // their positions
   uint32_t* crossings;
   float* partial;  // [chunks][2][hidden]: the sums of a chunk's first run (it began before) and of its last (it goes on)
@@ -380,33 +386,50 @@ struct Segments {
 };
 
 // One group of `1 << lane_bits` threads per chunk; a thread owns one vector column of it and has a batch of rows in
-// flight, with the table's rows that the batch completes where they are added to.
+// flight, with the table's rows that the batch completes where they are added to.  The chunks' keys and positions are
+// staged in shared memory first, so that only the rows themselves are waited for.
+constexpr int kStagedList = 4096;  // entries for all chunks of a CTA
+
 template <typename G, typename W, int VEC, bool ADD>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 3)
 sum_chunks(const __grid_constant__ Segments s, const G* __restrict__ grad_out, W* __restrict__ grad_table, float scale) {
   constexpr int kBatch = (int)sizeof(G) * VEC + (ADD ? (int)sizeof(W) * VEC : 0) <= 16 ? 8 : 4;
+  extern __shared__ uint32_t staged[];  // keys of the CTA's chunks and one behind them, then their positions
   dependent_launch_prologue();
-  const size_t chunk = (size_t)blockIdx.x * (kThreads >> s.lane_bits) + (threadIdx.x >> s.lane_bits);
+  const uint32_t groups = kThreads >> s.lane_bits, group = threadIdx.x >> s.lane_bits, entries = groups * s.chunk_length;
+  {
+    const size_t from = (size_t)blockIdx.x * entries;
+    for (uint32_t i = threadIdx.x; i <= entries; i += kThreads) {
+      const bool inside = from + i < s.count;
+      staged[i] = inside ? s.keys[from + i] : s.vocabulary;
+      if (i < entries) staged[entries + 1 + i] = inside ? s.order[from + i] : 0;
+    }
+  }
+  __syncthreads();
+  const size_t chunk = (size_t)blockIdx.x * groups + group;
   if (chunk >= s.chunks) return;
+  const uint32_t* keys = staged + group * s.chunk_length;
+  const uint32_t* order = staged + entries + 1 + group * s.chunk_length;
   const int lane = threadIdx.x & ((1 << s.lane_bits) - 1);
-  const size_t hidden = (size_t)s.steps * VEC;
-  const uint32_t first = (uint32_t)(chunk * s.chunk_length);
-  const bool first_began_before = first > 0 && s.keys[first - 1] == s.keys[first];
+  const size_t hidden = (size_t)s.steps * VEC, first = chunk * s.chunk_length;
+  const bool first_began_before = first > 0 && s.keys[first - 1] == keys[0];
   for (int step = (blockIdx.y << s.lane_bits) + lane; step < s.steps; step += gridDim.y << s.lane_bits) {
     const size_t column = (size_t)step * VEC;
+    const G* from = grad_out + column;
     bool began_before = first_began_before, open = false;
-    float sum[VEC] = {};
-    for (uint32_t at = first; at < first + s.chunk_length && at < s.count; at += kBatch) {
+    Sum<VEC> sum;
+    sum.clear();
+    for (uint32_t at = 0; at < s.chunk_length; at += kBatch) {
       uint32_t key[kBatch + 1];
 #pragma unroll
-      for (int j = 0; j <= kBatch; ++j) key[j] = s.keys[at + j];  // chunks are whole batches, the list has a tail
-      if (key[0] >= s.vocabulary) break;                         // dropped tokens, or the tail: nothing follows
+      for (int j = 0; j <= kBatch; ++j) key[j] = keys[at + j];
+      if (key[0] >= s.vocabulary) break;  // dropped tokens, or behind the list: nothing follows
       Pack<G, VEC> rows[kBatch];
       Pack<W, VEC> old[ADD ? kBatch : 1];
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
         if (key[j] < s.vocabulary) {
-          rows[j] = load_stream<G, VEC>(grad_out + (size_t)s.order[at + j] * hidden + column);
+          rows[j] = load_stream<G, VEC>(from + (size_t)order[at + j] * hidden);
           if constexpr (ADD) {
             if (key[j] != key[j + 1]) old[j] = load_stream<W, VEC>(grad_table + (size_t)key[j] * hidden + column);
           }
@@ -415,25 +438,21 @@ sum_chunks(const __grid_constant__ Segments s, const G* __restrict__ grad_out, W
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
         if (key[j] < s.vocabulary) {
-          float value[VEC];
-          widen<G, VEC>(rows[j], value);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) sum[e] += value[e];
+          sum.add(rows[j]);
           open = key[j] == key[j + 1];
           if (!open) {
             W* row = grad_table + (size_t)key[j] * hidden + column;
-            if (began_before) keep_partial<VEC>(s.partial + chunk * 2 * hidden + column, sum);
-            else if constexpr (ADD) add_to_row<W, VEC>(row, old[j], sum, scale);
-            else write_row<W, VEC>(row, sum, scale);
+            if (began_before) *reinterpret_cast<Pack<float, VEC>*>(s.partial + chunk * 2 * hidden + column) = sum.values();
+            else if constexpr (ADD) store_stream<W, VEC>(row, sum.times_plus(scale, old[j]));
+            else store_stream<W, VEC>(row, sum.template times<W>(scale));
             began_before = false;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) sum[e] = 0.0f;
+            sum.clear();
           }
         }
       }
     }
     if (open) {
-      keep_partial<VEC>(s.partial + (chunk * 2 + (began_before ? 0 : 1)) * hidden + column, sum);
+      *reinterpret_cast<Pack<float, VEC>*>(s.partial + (chunk * 2 + (began_before ? 0 : 1)) * hidden + column) = sum.values();
       if (!began_before && step == 0) s.crossings[1 + atomicAdd(s.crossings, 1u)] = (uint32_t)chunk;
     }
   }
@@ -445,7 +464,7 @@ sum_chunks(const __grid_constant__ Segments s, const G* __restrict__ grad_out, W
 template <typename W, int VEC, bool ADD>
 __global__ void __launch_bounds__(kThreads)
 join_and_fill(const __grid_constant__ Segments s, W* __restrict__ grad_table, float scale, unsigned join_blocks, const uint8_t* __restrict__ named) {
-  __shared__ float parts[kThreads / 32][32][VEC + 1];
+  __shared__ Pack<float, VEC> parts[kThreads / 32][32];
   dependent_launch_prologue();
   const size_t hidden = (size_t)s.steps * VEC;
   if (blockIdx.x >= join_blocks) {
@@ -473,27 +492,21 @@ join_and_fill(const __grid_constant__ Segments s, W* __restrict__ grad_table, fl
       end += found;
       more = found == kThreads;
     }
-    float sum[VEC] = {};
+    Sum<VEC> sum;
+    sum.clear();
     if (step < s.steps) {
-#pragma unroll 4
-      for (size_t c = chunk + slice; c < end; c += kThreads / 32) {
-        const float* from = s.partial + (c * 2 + (c == chunk ? 1 : 0)) * hidden + column;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) sum[e] += from[e];
-      }
+#pragma unroll 8
+      for (size_t c = chunk + slice; c < end; c += kThreads / 32)
+        sum.add(*reinterpret_cast<const Pack<float, VEC>*>(s.partial + (c * 2 + (c == chunk ? 1 : 0)) * hidden + column));
     }
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) parts[slice][lane][e] = sum[e];
+    parts[slice][lane] = sum.values();
     __syncthreads();
     if (slice == 0 && step < s.steps) {
 #pragma unroll
-      for (int w = 1; w < kThreads / 32; ++w) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) sum[e] += parts[w][lane][e];
-      }
+      for (int w = 1; w < kThreads / 32; ++w) sum.add(parts[w][lane]);
       W* row = grad_table + (size_t)key * hidden + column;
-      if constexpr (ADD) add_to_row<W, VEC>(row, load_stream<W, VEC>(row), sum, scale);
-      else write_row<W, VEC>(row, sum, scale);
+      if constexpr (ADD) store_stream<W, VEC>(row, sum.times_plus(scale, load_stream<W, VEC>(row)));
+      else store_stream<W, VEC>(row, sum.template times<W>(scale));
     }
     __syncthreads();
   }
@@ -513,9 +526,7 @@ inline size_t round_up(size_t n) { return (n + 255) & ~(size_t)255; }
 
 template <typename Id, int R>
 int launch_cluster_sort(const GradientCall& call, unsigned ctas, int passes, int digit_bits, const SortedList& list, uint8_t* named, cudaStream_t stream) {
-  if (int status = check_runtime(cudaFuncSetAttribute(sort_in_cluster<Id, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ClusterSort<R>)),
-                                 "cudaFuncSetAttribute(embedding_backward sort)"))
-    return status;
+  if (int status = allow_shared_memory<sort_in_cluster<Id, R>>((int)sizeof(ClusterSort<R>), "cudaFuncSetAttribute(embedding_backward sort)")) return status;
   launch_dependent_cluster(sort_in_cluster<Id, R>, dim3(ctas), dim3(kSortThreads), ctas, sizeof(ClusterSort<R>), stream,
                            static_cast<const Id*>(call.tokens), (uint32_t)call.count, (uint32_t)call.vocabulary, call.padding, passes, digit_bits,
                            (uint32_t)ctas, list, named, device_status_word());
@@ -572,14 +583,15 @@ template <typename G, typename W, int VEC, bool ADD> int gradient(const Gradient
   s.lane_bits = 2;
   while (s.lane_bits < 8 && ((size_t)1 << s.lane_bits) < steps) ++s.lane_bits;
   const size_t groups = kThreads >> s.lane_bits, columns = (steps + ((size_t)1 << s.lane_bits) - 1) >> s.lane_bits;
-  // short chunks while there are few tokens, so that the SMs have groups to run; four waves of groups otherwise, at least
-  // eight (one batch) and at most 512 tokens long
+  // short chunks while there are few tokens, so that the SMs have groups to run; about four waves of groups otherwise, and
+  // no more of them than a CTA can stage
   const size_t resident = ((size_t)multiprocessor_count() * 1024) >> s.lane_bits;
-  s.chunk_length = 8;
-  while (s.chunk_length < 512 && count * columns > (size_t)s.chunk_length * resident * 4) s.chunk_length *= 2;
+  s.chunk_length = count <= 2048 ? 8 : count <= 8192 ? 16 : 32;
+  while (2 * s.chunk_length * groups <= (size_t)kStagedList && s.chunk_length < 512 && count * columns > (size_t)s.chunk_length * resident * 4)
+    s.chunk_length *= 2;
   s.chunks = (uint32_t)((count + s.chunk_length - 1) / s.chunk_length);
   const bool spare = count > 65536;
-  const size_t list = round_up((count + kListTail) * 4), crossings = round_up((1 + (size_t)s.chunks) * 4);
+  const size_t list = round_up(count * 4), crossings = round_up((1 + (size_t)s.chunks) * 4);
   const size_t counts_bytes = spare ? round_up((count + kTile - 1) / kTile * kBins * 4) : 0, partial = round_up((size_t)s.chunks * 2 * call.hidden * 4);
   const size_t named_bytes = ADD ? 0 : round_up(call.vocabulary);
   Workspace workspace(stream);
@@ -612,7 +624,8 @@ template <typename G, typename W, int VEC, bool ADD> int gradient(const Gradient
   s.crossings = sorted.crossings;
   W* table = static_cast<W*>(call.grad_table);
   launch_dependent(sum_chunks<G, W, VEC, ADD>, dim3((unsigned)((s.chunks + groups - 1) / groups), (unsigned)(columns < 65535 ? columns : 65535)),
-                   dim3(kThreads), 0, stream, s, static_cast<const G*>(call.grad_out), table, call.scale);
+                   dim3(kThreads), (2 * groups * s.chunk_length + 1) * sizeof(uint32_t), stream, s, static_cast<const G*>(call.grad_out), table,
+                   call.scale);
   if (int status = check_launch("embedding_backward sum launch")) return status;
   // at most one run crosses each border between two chunks
   const size_t most_items = (size_t)(s.chunks - 1) * ((steps + 31) / 32), join_most = (size_t)multiprocessor_count() * 4;

@@ -236,13 +236,13 @@ template <typename T> int join(const Backward<T>& p, int shares, void* grad_weig
 }
 
 template <typename T, typename Rows, bool RESIDUAL> int launch_rows(Backward<T> p, void* grad_weight, void* grad_bias, cudaStream_t stream) {
-  const auto kernel = norm_backward_rows<T, Rows, RESIDUAL>;
+  constexpr auto kernel = norm_backward_rows<T, Rows, RESIDUAL>;
   const size_t wanted = (p.rows + Rows::GROUPS - 1) / Rows::GROUPS, most = (size_t)multiprocessor_count();
   const int blocks = (int)(wanted < most ? wanted : most);
   Workspace workspace(stream);
   if (int status = workspace.take((size_t)blocks * 2 * p.hidden * sizeof(float), "layernorm_backward workspace")) return status;
   p.partial = reinterpret_cast<float*>(workspace.data());
-  if (int status = check_runtime(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Rows::kBytes), "cudaFuncSetAttribute(layernorm_backward)"))
+  if (int status = allow_shared_memory<kernel>(Rows::kBytes, "cudaFuncSetAttribute(layernorm_backward)"))
     return status;
   launch_dependent(kernel, dim3(blocks), dim3(kRowThreads), (size_t)Rows::kBytes, stream, p);
   if (int status = check_launch("layernorm_backward kernel launch")) return status;

@@ -308,8 +308,8 @@ norm_rows_by_element(const __grid_constant__ Forward<T> p) {
 }
 
 template <typename T, typename Rows, bool RESIDUAL> int launch_rows(const Forward<T>& p, cudaStream_t stream) {
-  const auto kernel = norm_rows<T, Rows, RESIDUAL>;
-  if (int status = check_runtime(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Rows::kBytes), "cudaFuncSetAttribute(layernorm_forward)"))
+  constexpr auto kernel = norm_rows<T, Rows, RESIDUAL>;
+  if (int status = allow_shared_memory<kernel>(Rows::kBytes, "cudaFuncSetAttribute(layernorm_forward)"))
     return status;
   const size_t wanted = (p.rows + Rows::GROUPS - 1) / Rows::GROUPS, most = (size_t)multiprocessor_count();
   launch_dependent(kernel, dim3((unsigned)(wanted < most ? wanted : most)), dim3(kRowThreads), (size_t)Rows::kBytes, stream, p);
@@ -368,8 +368,7 @@ template <typename T> int forward(const Forward<T>& p, bool aligned, cudaStream_
   }
   const int smem = p.hidden * (int)sizeof(float);
   if (smem > 48 * 1024) {
-    if (int status = check_runtime(cudaFuncSetAttribute(norm_rows_by_element<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 32768 * 4),
-                                   "cudaFuncSetAttribute(layernorm_forward)"))
+    if (int status = allow_shared_memory<norm_rows_by_element<T>>(32768 * 4, "cudaFuncSetAttribute(layernorm_forward)"))
       return status;
   }
   launch_dependent(norm_rows_by_element<T>, dim3((unsigned)p.rows), dim3(kElementThreads), (size_t)smem, stream, p);

@@ -216,13 +216,10 @@ class CompiledKernel:
                 "(baybridge_b200 has no CPU runtime)"
             )
         stream = kwargs.get("stream") if kwargs else None
-        for arg in args:
-            if type(arg) is not TensorHandle:
-                break
-        else:
-            # the hot call: device tensor handles only (plus stream=) need no normalisation
-            if not kwargs or (len(kwargs) == 1 and "stream" in kwargs):
-                return self.runtime_callable(*args, **kwargs)
+        # the hot call: device tensor handles (or groups of them) as they were compiled for need no normalisation
+        quick = getattr(self.runtime_callable, "quick", None)
+        if quick is not None and (not kwargs or (len(kwargs) == 1 and "stream" in kwargs)) and quick(args, stream):
+            return None
         args = tuple(normalize_runtime_argument(arg, stream=stream) for arg in args)
         kwargs = {
             name: value if name == "stream" else normalize_runtime_argument(value, stream=stream)
@@ -271,12 +268,22 @@ def _bind_user_arguments(definition, backend_launcher: Callable[..., Any], bindi
     direct = (len(positional) == len(parameters) and "stream" not in signature.parameters
               and all(not binding["path"] and binding["parameter"] in positional for binding in bindings))
     order = [positional.index(binding["parameter"]) for binding in bindings] if direct else []
-    # a backend launcher that takes whole tensor groups (one argument for a list of leaves) is offered them first:
-    # per parameter that has leaves, its place in the call and the position of its first leaf
+    # a backend launcher may offer two short cuts, which return False where the ordinary path has to look closer (and find
+    # the error): ``quick(leaves, stream)``, and ``grouped(values, stream)`` for lists of leaves given as one tensor
+    # group each (``values``: the argument of every parameter by the position of its first leaf)
     flat = all(binding["parameter"] in positional and len(binding["path"]) <= 1 for binding in bindings)
-    grouped = getattr(backend_launcher, "grouped", None) if flat else None
+    quick_leaves = getattr(backend_launcher, "quick", None) if direct else None
+    grouped = getattr(backend_launcher, "grouped", None) if flat and not direct else None
     spans = [(positional.index(binding["parameter"]), leaf) for leaf, binding in enumerate(bindings)
              if grouped is not None and binding["path"] in ([], [0])]
+    every = order == list(range(len(positional)))
+
+    def quick(args: tuple[Any, ...], stream: Any) -> bool:
+        if len(args) != len(positional):
+            return False
+        if quick_leaves is not None:
+            return quick_leaves(args if every else [args[index] for index in order], stream)
+        return grouped({leaf: args[place] for place, leaf in spans}, stream)
 
     def launcher(*args: Any, **kwargs: Any) -> Any:
         if direct and len(args) == len(positional) and (not kwargs or (len(kwargs) == 1 and "stream" in kwargs)):
@@ -287,9 +294,8 @@ def _bind_user_arguments(definition, backend_launcher: Callable[..., Any], bindi
                     leaves = [normalize_runtime_argument(value, stream=stream) for value in leaves]
                     break
             return backend_launcher(*leaves) if stream is None else backend_launcher(*leaves, stream=stream)
-        if grouped is not None and len(args) == len(positional) and not kwargs.keys() - {"stream"}:
-            if grouped({leaf: args[place] for place, leaf in spans}, kwargs.get("stream")):
-                return None
+        if grouped is not None and not kwargs.keys() - {"stream"} and quick(args, kwargs.get("stream")):
+            return None
         stream = None if "stream" in signature.parameters else kwargs.pop("stream", None)
         bound = signature.bind_partial(*args, **kwargs).arguments
         if stream is None and "stream" in bound:
@@ -300,6 +306,8 @@ def _bind_user_arguments(definition, backend_launcher: Callable[..., Any], bindi
         ]
         return backend_launcher(*leaves) if stream is None else backend_launcher(*leaves, stream=stream)
 
+    if quick_leaves is not None or grouped is not None:
+        launcher.quick = quick  # type: ignore[attr-defined]
     return launcher
 
 

@@ -311,6 +311,8 @@ class TensorHandle:
         object.__setattr__(self, "dtype", normalize_dtype_name(str(self.dtype)))
         if self.stride is not None:
             object.__setattr__(self, "stride", tuple(int(step) for step in self.stride))
+        # what a launcher compares per argument and call, in one piece: dtype, shape, device type, whether it is dense
+        object.__setattr__(self, "signature", (self.dtype, self.shape, int(self.device_type), self.is_contiguous))
 
     def mark_layout_dynamic(self, leading_dim: int | None = None) -> "TensorHandle":
         if leading_dim is not None and not 0 <= leading_dim < len(self.shape):
