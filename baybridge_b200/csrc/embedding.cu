@@ -221,9 +221,11 @@ __device__ __forceinline__ uint32_t in_cta(const void* shared, uint32_t rank) {
   return a;
 }
 
-// Up to 65536 tokens in one launch: one cluster of 1, 2, 4 or 8 CTAs holds them all in shared memory.  Every pass ranks in
+// Up to 65536 tokens in one launch: one cluster of up to 16 CTAs holds them all in shared memory.  Every pass ranks in
 // each CTA, adds up the CTAs' digit counts through distributed shared memory and sends every element to its place there;
 // nobody touches another CTA's memory after the last pass's barrier.
+constexpr uint32_t kMostCtas = 16;
+
 template <int R> struct ClusterSort {
   uint2 pairs[kSortThreads * R];
   uint32_t counters[kSortWarps][kCounterWords];
@@ -259,11 +261,16 @@ sort_in_cluster(const Id* __restrict__ tokens, uint32_t count, uint32_t vocabula
     uint32_t total = 0, earlier = 0;
     if (ctas > 1) cluster_barrier();  // every CTA's totals stand
     if (threadIdx.x < kBins) {
-      for (uint32_t c = 0; c < ctas; ++c) {
-        uint32_t n;
-        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(n) : "r"(in_cta(&s.totals[threadIdx.x], c)) : "memory");
-        if (c < rank_of_cta) earlier += n;
-        total += n;
+      uint32_t n[kMostCtas];  // all of them on their way at once
+#pragma unroll
+      for (uint32_t c = 0; c < kMostCtas; ++c) {
+        n[c] = 0;
+        if (c < ctas) asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(n[c]) : "r"(in_cta(&s.totals[threadIdx.x], c)) : "memory");
+      }
+#pragma unroll
+      for (uint32_t c = 0; c < kMostCtas; ++c) {
+        if (c < rank_of_cta) earlier += n[c];
+        total += n[c];
       }
     }
     const uint32_t start = exclusive_over_bins(total, s.warp_totals) + earlier;
@@ -461,20 +468,30 @@ sum_chunks(const __grid_constant__ Segments s, const G* __restrict__ grad_out, W
 // Two jobs in one launch.  The first `join_blocks` CTAs join the partial sums of the runs that cross a chunk's border: 32
 // vector columns of one run at a time, eight warps over its chunks, added up in a fixed order.  The other CTAs, where the
 // whole table is written, fill the rows that no token names with zeros; the joins hide behind them.
+constexpr int kFillRows = 4;  // rows that a group looks at together
+
 template <typename W, int VEC, bool ADD>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, ADD ? 4 : 6)
 join_and_fill(const __grid_constant__ Segments s, W* __restrict__ grad_table, float scale, unsigned join_blocks, const uint8_t* __restrict__ named) {
   __shared__ Pack<float, VEC> parts[kThreads / 32][32];
   dependent_launch_prologue();
   const size_t hidden = (size_t)s.steps * VEC;
   if (blockIdx.x >= join_blocks) {
-    const size_t row = (size_t)(blockIdx.x - join_blocks) * (kThreads >> s.lane_bits) + (threadIdx.x >> s.lane_bits);
-    if (row >= s.vocabulary || named[row]) return;
+    const int lanes = 1 << s.lane_bits, groups = kThreads >> s.lane_bits;
+    const size_t first = (size_t)(blockIdx.x - join_blocks) * groups * kFillRows + (threadIdx.x >> s.lane_bits);
+    bool empty[kFillRows];
+#pragma unroll
+    for (int r = 0; r < kFillRows; ++r) empty[r] = first + r * groups < s.vocabulary && !named[first + r * groups];
     Pack<W, VEC> zero;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) zero.v[e] = Conv<float, W>::narrow(0.0f);
-    const int lanes = 1 << s.lane_bits;
-    for (int step = threadIdx.x & (lanes - 1); step < s.steps; step += lanes) store_stream<W, VEC>(grad_table + (row * s.steps + step) * VEC, zero);
+#pragma unroll
+    for (int r = 0; r < kFillRows; ++r) {
+      if (empty[r]) {
+        W* row = grad_table + (first + r * groups) * ((size_t)s.steps * VEC);
+        for (int step = threadIdx.x & (lanes - 1); step < s.steps; step += lanes) store_stream<W, VEC>(row + (size_t)step * VEC, zero);
+      }
+    }
     return;
   }
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
@@ -526,6 +543,11 @@ inline size_t round_up(size_t n) { return (n + 255) & ~(size_t)255; }
 
 template <typename Id, int R>
 int launch_cluster_sort(const GradientCall& call, unsigned ctas, int passes, int digit_bits, const SortedList& list, uint8_t* named, cudaStream_t stream) {
+  if (ctas > 8) {  // beyond the portable size; the attribute is cheap to set again
+    if (int status = check_runtime(cudaFuncSetAttribute(sort_in_cluster<Id, R>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
+                                   "cudaFuncSetAttribute(embedding_backward sort)"))
+      return status;
+  }
   if (int status = allow_shared_memory<sort_in_cluster<Id, R>>((int)sizeof(ClusterSort<R>), "cudaFuncSetAttribute(embedding_backward sort)")) return status;
   launch_dependent_cluster(sort_in_cluster<Id, R>, dim3(ctas), dim3(kSortThreads), ctas, sizeof(ClusterSort<R>), stream,
                            static_cast<const Id*>(call.tokens), (uint32_t)call.count, (uint32_t)call.vocabulary, call.padding, passes, digit_bits,
@@ -541,12 +563,15 @@ int sort_tokens(const GradientCall& call, const SortedList& list, const SortedLi
   int bits = 1;  // of the keys 0 .. vocabulary
   while (((unsigned long long)call.vocabulary >> bits) != 0) ++bits;
   const int passes = (bits + kDigitBits - 1) / kDigitBits, digit_bits = (bits + passes - 1) / passes;
-  if (count <= 1024) return launch_cluster_sort<Id, 1>(call, 1, passes, digit_bits, list, named, stream);
-  if (count <= 4096) return launch_cluster_sort<Id, 4>(call, 1, passes, digit_bits, list, named, stream);
-  if (count <= 8192) return launch_cluster_sort<Id, 4>(call, 2, passes, digit_bits, list, named, stream);
-  if (count <= 16384) return launch_cluster_sort<Id, 4>(call, 4, passes, digit_bits, list, named, stream);
-  if (count <= 32768) return launch_cluster_sort<Id, 4>(call, 8, passes, digit_bits, list, named, stream);
-  if (count <= 65536) return launch_cluster_sort<Id, 8>(call, 8, passes, digit_bits, list, named, stream);
+  const auto ctas = [count](uint32_t each) {  // a power of two
+    unsigned n = 1;
+    while (n * each < count) n *= 2;
+    return n;
+  };
+  // Few elements a thread and many CTAs: 65536 tokens 24 us with 16 CTAs, 35 us with eight of twice the elements.
+  if (count <= 16384) return launch_cluster_sort<Id, 1>(call, ctas(1024), passes, digit_bits, list, named, stream);
+  if (count <= 32768) return launch_cluster_sort<Id, 2>(call, ctas(2048), passes, digit_bits, list, named, stream);
+  if (count <= 65536) return launch_cluster_sort<Id, 4>(call, ctas(4096), passes, digit_bits, list, named, stream);
   const Id* tokens = static_cast<const Id*>(call.tokens);
   const int tiles = (int)((call.count + kTile - 1) / kTile);
   const uint32_t mask = (1u << digit_bits) - 1;
@@ -586,7 +611,7 @@ template <typename G, typename W, int VEC, bool ADD> int gradient(const Gradient
   // short chunks while there are few tokens, so that the SMs have groups to run; about four waves of groups otherwise, and
   // no more of them than a CTA can stage
   const size_t resident = ((size_t)multiprocessor_count() * 1024) >> s.lane_bits;
-  s.chunk_length = count <= 2048 ? 8 : count <= 8192 ? 16 : 32;
+  s.chunk_length = count <= 4096 ? 8 : 16;
   while (2 * s.chunk_length * groups <= (size_t)kStagedList && s.chunk_length < 512 && count * columns > (size_t)s.chunk_length * resident * 4)
     s.chunk_length *= 2;
   s.chunks = (uint32_t)((count + s.chunk_length - 1) / s.chunk_length);
@@ -628,9 +653,9 @@ template <typename G, typename W, int VEC, bool ADD> int gradient(const Gradient
                    call.scale);
   if (int status = check_launch("embedding_backward sum launch")) return status;
   // at most one run crosses each border between two chunks
-  const size_t most_items = (size_t)(s.chunks - 1) * ((steps + 31) / 32), join_most = (size_t)multiprocessor_count() * 4;
+  const size_t most_items = (size_t)(s.chunks - 1) * ((steps + 31) / 32), join_most = (size_t)multiprocessor_count() * 8;
   const unsigned join_blocks = (unsigned)(most_items < join_most ? most_items : join_most);
-  const unsigned fill_blocks = named ? (unsigned)((call.vocabulary + groups - 1) / groups) : 0;
+  const unsigned fill_blocks = named ? (unsigned)((call.vocabulary + groups * kFillRows - 1) / (groups * kFillRows)) : 0;
   if (join_blocks + fill_blocks > 0) {
     launch_dependent(join_and_fill<W, VEC, ADD>, dim3(join_blocks + fill_blocks), dim3(kThreads), 0, stream, s, table, call.scale, join_blocks,
                      static_cast<const uint8_t*>(named));
