@@ -10,8 +10,8 @@
 // memory.  All arithmetic is fp32; 1 - beta^step is -expm1(step log beta), which keeps its digits for beta near 1.
 #include <math.h>
 
-#include "bb200_elementwise.cuh"
 #include "bb200_internal.h"
+#include "bb200_rows.cuh"
 
 namespace bb200 {
 namespace {
@@ -26,7 +26,7 @@ struct Entry {
   float* master;
   unsigned long long numel;
   float decay;
-  int vector_ok;  // every tensor 16-byte aligned
+  int access;  // 2: tensors aligned to a thread's eight elements (16 or 32 bytes); 1: to 16 bytes; 0: less
 };
 
 // Kernel parameters hold at most 32764 bytes; the small table keeps the parameter block of ordinary calls short.
@@ -42,11 +42,15 @@ static_assert(sizeof(Table<kLargeTable>) <= 32764, "the table has to fit the ker
 
 struct Step {
   float rate, factor, beta1, beta2, one_minus_beta1, one_minus_beta2, inverse1, inverse2, epsilon;
-  __device__ __forceinline__ void update(float grad, float decay_factor, float& value, float& m, float& v) const {
-    const float g = grad * factor;
-    m = fmaf(beta1, m, one_minus_beta1 * g);
-    v = fmaf(beta2, v, one_minus_beta2 * g * g);
-    value = fmaf(-rate, (m * inverse1) / (sqrtf(v * inverse2) + epsilon), value * decay_factor);
+  // two elements
+  __device__ __forceinline__ void update(F2 grad, F2 decay_factor, F2& value, F2& m, F2& v) const {
+    const F2 g = grad * both(factor);
+    m = fma2(both(beta1), m, both(one_minus_beta1) * g);
+    v = fma2(both(beta2), v, both(one_minus_beta2) * g * g);
+    float m_low, m_high, v_low, v_high;
+    split(m * both(inverse1), m_low, m_high);
+    split(v * both(inverse2), v_low, v_high);
+    value = fma2(both(-rate), make_f2(m_low / (sqrtf(v_low) + epsilon), m_high / (sqrtf(v_high) + epsilon)), value * decay_factor);
   }
 };
 
@@ -66,17 +70,17 @@ adamw_step(const __grid_constant__ Table<CAPACITY> table) {
   const unsigned long long at = base + threadIdx.x * kVec;
   P* param = static_cast<P*>(entry.param);
   const G* grad = static_cast<const G*>(entry.grad);
-  const bool whole = entry.vector_ok && at + kVec <= entry.numel;
+  const bool whole = entry.access && at + kVec <= entry.numel, wide = entry.access == 2;
   // the tile's loads are issued before anything waits for the schedule
   Pack<P, kVec> p;
   Pack<G, kVec> g;
   Pack<float, kVec> m, v, master;
   if (whole) {
-    g = load_stream<G, kVec>(grad + at);
-    m = load_stream<float, kVec>(entry.exp_avg + at);
-    v = load_stream<float, kVec>(entry.exp_avg_sq + at);
-    if constexpr (MASTERS) master = load_stream<float, kVec>(entry.master + at);
-    else p = load_stream<P, kVec>(param + at);
+    g = load_stream_32<G, kVec>(grad + at, wide);
+    m = load_stream_32<float, kVec>(entry.exp_avg + at, wide);
+    v = load_stream_32<float, kVec>(entry.exp_avg_sq + at, wide);
+    if constexpr (MASTERS) master = load_stream_32<float, kVec>(entry.master + at, wide);
+    else p = load_stream_32<P, kVec>(param + at, wide);
   }
   const float rate = table.schedule[0], count = table.schedule[1], factor = table.schedule[2];
   if (threadIdx.x == 0) corrections[0] = -1.0f / expm1f(count * table.log_beta1);
@@ -87,28 +91,35 @@ adamw_step(const __grid_constant__ Table<CAPACITY> table) {
   const float decay_factor = 1.0f - rate * entry.decay;
   if (whole) {
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      float value = MASTERS ? master.v[e] : Conv<float, P>::widen(p.v[e]);
-      step.update(Conv<float, G>::widen(g.v[e]), decay_factor, value, m.v[e], v.v[e]);
-      if constexpr (MASTERS) master.v[e] = value;
-      p.v[e] = Conv<float, P>::narrow(value);
+    for (int i = 0; i < kVec / 2; ++i) {
+      F2 value = MASTERS ? Pairs<float>::get(master, i) : Pairs<P>::get(p, i);
+      F2 m_pair = Pairs<float>::get(m, i), v_pair = Pairs<float>::get(v, i);
+      step.update(Pairs<G>::get(g, i), both(decay_factor), value, m_pair, v_pair);
+      Pairs<float>::set(m, i, m_pair);
+      Pairs<float>::set(v, i, v_pair);
+      if constexpr (MASTERS) Pairs<float>::set(master, i, value);
+      Pairs<P>::set(p, i, value);
     }
-    store_stream<float, kVec>(entry.exp_avg + at, m);
-    store_stream<float, kVec>(entry.exp_avg_sq + at, v);
-    if constexpr (MASTERS) store_stream<float, kVec>(entry.master + at, master);
-    store_stream<P, kVec>(param + at, p);
+    store_stream_32<float, kVec>(entry.exp_avg + at, m, wide);
+    store_stream_32<float, kVec>(entry.exp_avg_sq + at, v, wide);
+    if constexpr (MASTERS) store_stream_32<float, kVec>(entry.master + at, master, wide);
+    store_stream_32<P, kVec>(param + at, p, wide);
   }
   // the ragged end of a tensor, or tensors that are not 16-byte aligned: neighbouring threads take neighbouring elements
   const unsigned long long tile_end = base + kTileElements < entry.numel ? base + kTileElements : entry.numel;
-  const unsigned long long first = entry.vector_ok ? tile_end - tile_end % kVec : base;
+  const unsigned long long first = entry.access ? tile_end - tile_end % kVec : base;
   for (unsigned long long i = first + threadIdx.x; i < tile_end; i += kThreads) {
-    float value = MASTERS ? entry.master[i] : Conv<float, P>::widen(param[i]);
-    float one_m = entry.exp_avg[i], one_v = entry.exp_avg_sq[i];
-    step.update(Conv<float, G>::widen(grad[i]), decay_factor, value, one_m, one_v);
-    entry.exp_avg[i] = one_m;
-    entry.exp_avg_sq[i] = one_v;
-    if constexpr (MASTERS) entry.master[i] = value;
-    param[i] = Conv<float, P>::narrow(value);
+    F2 value = both(MASTERS ? entry.master[i] : Conv<float, P>::widen(param[i]));
+    F2 one_m = both(entry.exp_avg[i]), one_v = both(entry.exp_avg_sq[i]);
+    step.update(both(Conv<float, G>::widen(grad[i])), both(decay_factor), value, one_m, one_v);
+    float low, unused;
+    split(one_m, low, unused);
+    entry.exp_avg[i] = low;
+    split(one_v, low, unused);
+    entry.exp_avg_sq[i] = low;
+    split(value, low, unused);
+    if constexpr (MASTERS) entry.master[i] = low;
+    param[i] = Conv<float, P>::narrow(low);
   }
 }
 
@@ -165,8 +176,12 @@ int launch_pair(const Call& call, int param_code, int grad_code, cudaStream_t st
     entry.master = MASTERS ? static_cast<float*>(call.masters[i]) : nullptr;
     entry.numel = call.numels[i];
     entry.decay = call.decays[i];
-    entry.vector_ok = aligned16(entry.param) && aligned16(entry.grad) && aligned16(entry.exp_avg) && aligned16(entry.exp_avg_sq) &&
-                      (!MASTERS || aligned16(entry.master));
+    const auto vector = [](const void* p, size_t size) { return size == 4 ? aligned32(p) : aligned16(p); };
+    const bool sixteen = aligned16(entry.param) && aligned16(entry.grad) && aligned16(entry.exp_avg) && aligned16(entry.exp_avg_sq) &&
+                         (!MASTERS || aligned16(entry.master));
+    const bool whole = vector(entry.param, sizeof(P)) && vector(entry.grad, sizeof(G)) && aligned32(entry.exp_avg) &&
+                       aligned32(entry.exp_avg_sq) && (!MASTERS || aligned32(entry.master));
+    entry.access = whole ? 2 : sixteen ? 1 : 0;
     table.first_tile[table.count++] = (unsigned)tiles;
     tiles += more;
   }

@@ -64,6 +64,8 @@ __device__ __forceinline__ void dependent_launch_prologue() {
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+inline bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
+
 inline size_t dtype_bytes(bb200_dtype t) {
   switch (t) {
     case BB200_F32: case BB200_I32: return 4;
