@@ -102,6 +102,22 @@ template <typename T, int VEC> __device__ __forceinline__ void store_stream_32(T
   store_stream<T, VEC>(p, v);
 }
 
+// ---- clusters ----------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// The address of CTA `rank`'s copy of a shared variable of this CTA.
+__device__ __forceinline__ uint32_t in_cta(const void* shared, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(shared)), "r"(rank));
+  return a;
+}
+
 // ---- copies ahead ------------------------------------------------------------------------------------------------
 // 16 bytes from global to shared memory, both 16-byte aligned, of which `bytes` are read and the rest become zeros.
 __device__ __forceinline__ void copy_async_16(void* shared, const void* global) {

@@ -223,21 +223,6 @@ struct SortedList {
   uint32_t* crossings;  // [0]: how many runs cross a chunk's border (set to 0 here), then their first chunks
 };
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-}
-// The address of CTA `rank`'s copy of a shared variable of this CTA.
-__device__ __forceinline__ uint32_t in_cta(const void* shared, uint32_t rank) {
-  uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(shared)), "r"(rank));
-  return a;
-}
-
 // Up to 65536 tokens in one launch: one cluster of up to 16 CTAs holds them all in shared memory.  Every pass ranks in
 // each CTA, adds up the CTAs' digit counts through distributed shared memory and sends every element to its place there;
 // nobody touches another CTA's memory after the last pass's barrier.

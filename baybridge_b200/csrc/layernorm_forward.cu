@@ -262,49 +262,71 @@ norm_long_rows(const __grid_constant__ Forward<T> p) {
   }
 }
 
-// Tensors that do not start on a 16-byte boundary, and long rows of no whole vectors: element by element, the row kept in
-// shared memory as fp32.
-constexpr int kElementThreads = 256;
-template <typename T>
-__global__ void __launch_bounds__(kElementThreads)
+// Rows of any width and alignment, a brief CTA for ROWS of them: thread `lane` of LANES owns the columns lane, lane + LANES,
+// ..., and keeps them in registers; SURE of its COLUMNS lie inside every row this form is used for and are not asked about.
+template <typename T, int LANES, int ROWS, int COLUMNS, int SURE, bool RESIDUAL>
+__global__ void __launch_bounds__(LANES * ROWS)
 norm_rows_by_element(const __grid_constant__ Forward<T> p) {
-  extern __shared__ float row_values[];
-  __shared__ RowSums<kElementThreads, 1> scratch;
+  __shared__ RowSums<LANES, 1> scratch[ROWS];
   dependent_launch_prologue();
-  const size_t row = blockIdx.x, offset = row * (size_t)p.hidden;
+  const int group = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+  const size_t row = (size_t)blockIdx.x * ROWS + group;
+  if (row >= p.rows) return;
+  const size_t offset = row * (size_t)p.hidden + lane;
   const float scale = 1.0f / (float)p.hidden;
-  int turn = 0;
-  float sum = 0.0f;
-#pragma unroll 4
-  for (int c = threadIdx.x; c < p.hidden; c += kElementThreads) {
-    float v = Conv<float, T>::widen(p.x[offset + c]);
-    if (p.residual) {
-      v += Conv<float, T>::widen(p.residual[offset + c]);
-      p.out_resid[offset + c] = Conv<float, T>::narrow(v);
+  const auto has = [&](int k) { return k < SURE || lane + k * LANES < p.hidden; };
+  float s[COLUMNS];
+  T a[COLUMNS], b[COLUMNS];
+#pragma unroll
+  for (int k = 0; k < COLUMNS; ++k) {
+    if (has(k)) {
+      a[k] = p.x[offset + k * LANES];
+      if constexpr (RESIDUAL) b[k] = p.residual[offset + k * LANES];
     }
-    row_values[c] = v;  // read back by this thread only
-    sum += v;
   }
-  float sums[1] = {sum};
-  row_sums<kElementThreads>(sums, &scratch, turn, 1);
-  const float mean = sums[0] * scale;
-  float centred = 0.0f;
-  for (int c = threadIdx.x; c < p.hidden; c += kElementThreads) {
-    const float d = row_values[c] - mean;
-    centred = fmaf(d, d, centred);
+  float sum[1] = {0.0f};
+#pragma unroll
+  for (int k = 0; k < COLUMNS; ++k) {
+    s[k] = has(k) ? Conv<float, T>::widen(a[k]) : 0.0f;
+    if constexpr (RESIDUAL) {
+      if (has(k)) {
+        s[k] += Conv<float, T>::widen(b[k]);
+        p.out_resid[offset + k * LANES] = Conv<float, T>::narrow(s[k]);
+      }
+    }
+    sum[0] += s[k];
   }
-  sums[0] = centred;
-  row_sums<kElementThreads>(sums, &scratch, turn, 1);
-  const float rstd = 1.0f / sqrtf(sums[0] * scale + p.epsilon);
-  if (threadIdx.x == 0) {
+  int turn = 0;
+  row_sums<LANES>(sum, &scratch[group], turn, group);
+  const float mean = sum[0] * scale;
+  sum[0] = 0.0f;
+#pragma unroll
+  for (int k = 0; k < COLUMNS; ++k) {
+    s[k] -= mean;
+    if (has(k)) sum[0] = fmaf(s[k], s[k], sum[0]);
+  }
+  row_sums<LANES>(sum, &scratch[group], turn, group);
+  const float rstd = 1.0f / sqrtf(sum[0] * scale + p.epsilon);
+  if (lane == 0) {
     p.mean[row] = mean;
     p.rstd[row] = rstd;
   }
-  for (int c = threadIdx.x; c < p.hidden; c += kElementThreads) {
-    const float w = p.wide ? static_cast<const float*>(p.weight)[c] : Conv<float, T>::widen(static_cast<const T*>(p.weight)[c]);
-    const float b = !p.bias ? 0.0f : p.wide ? static_cast<const float*>(p.bias)[c] : Conv<float, T>::widen(static_cast<const T*>(p.bias)[c]);
-    p.out[offset + c] = Conv<float, T>::narrow(fmaf((row_values[c] - mean) * rstd, w, b));
+#pragma unroll
+  for (int k = 0; k < COLUMNS; ++k) {
+    if (has(k)) {
+      const int c = lane + k * LANES;
+      const float w = p.wide ? static_cast<const float*>(p.weight)[c] : Conv<float, T>::widen(static_cast<const T*>(p.weight)[c]);
+      const float v = !p.bias ? 0.0f : p.wide ? static_cast<const float*>(p.bias)[c] : Conv<float, T>::widen(static_cast<const T*>(p.bias)[c]);
+      p.out[offset + k * LANES] = Conv<float, T>::narrow(fmaf(s[k] * rstd, w, v));
+    }
   }
+}
+
+template <typename T, int LANES, int ROWS, int COLUMNS, int SURE> int launch_by_element(const Forward<T>& p, cudaStream_t stream) {
+  const dim3 grid((unsigned)((p.rows + ROWS - 1) / ROWS)), block(LANES * ROWS);
+  if (p.residual) launch_dependent(norm_rows_by_element<T, LANES, ROWS, COLUMNS, SURE, true>, grid, block, 0, stream, p);
+  else launch_dependent(norm_rows_by_element<T, LANES, ROWS, COLUMNS, SURE, false>, grid, block, 0, stream, p);
+  return check_launch("layernorm_forward kernel launch");
 }
 
 template <typename T, typename Rows, bool RESIDUAL> int launch_rows(const Forward<T>& p, cudaStream_t stream) {
@@ -352,27 +374,29 @@ template <typename T> int forward(const Forward<T>& p, bool aligned, cudaStream_
     else launch_dependent(norm_long_rows<T, 1024, 4>, dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
     return check_launch("layernorm_forward kernel launch");
   }
-  if (aligned) {
-#define BB200_SHIFTED_ROWS(LANES, COLUMNS, SURE)                                                       \
+  // Other rows: a brief CTA for a few of them takes the fewest microseconds, the persistent form moves more bytes a second
+  // once there are many (4099 x 1535 f16: 10 us brief, 13 us persistent; 65536 x 1001 bf16 with residual: 141 and 112 us; 65536 x
+  // 65: 15 and 24 us).
+  if (aligned && p.hidden > 256 && p.rows * (size_t)p.hidden > ((size_t)1 << 24)) {
+#define BB200_SHIFTED_ROWS(LANES, COLUMNS, SURE)                                                    \
   if (p.hidden <= (LANES) * (COLUMNS))                                                             \
     return p.residual ? launch_rows<T, ShiftedRows<T, kRowThreads, LANES, COLUMNS, SURE, 2, 1, kMostSmem>, true>(p, stream) : launch_rows<T, ShiftedRows<T, kRowThreads, LANES, COLUMNS, SURE, 1, 1, kMostSmem>, false>(p, stream)
-    constexpr int kColumns = 16;
-    BB200_SHIFTED_ROWS(32, 4, 0);
-    BB200_SHIFTED_ROWS(32, kColumns / 2, 4);
-    BB200_SHIFTED_ROWS(32, kColumns, kColumns / 2);
-    BB200_SHIFTED_ROWS(64, kColumns, kColumns / 2);
-    BB200_SHIFTED_ROWS(128, kColumns, kColumns / 2);
-    BB200_SHIFTED_ROWS(256, kColumns, kColumns / 2);
-    BB200_SHIFTED_ROWS(512, kColumns, kColumns / 2);
+    BB200_SHIFTED_ROWS(32, 16, 8);
+    BB200_SHIFTED_ROWS(64, 16, 8);
+    BB200_SHIFTED_ROWS(128, 16, 8);
+    BB200_SHIFTED_ROWS(256, 16, 8);
+    BB200_SHIFTED_ROWS(512, 16, 8);
 #undef BB200_SHIFTED_ROWS
   }
-  const int smem = p.hidden * (int)sizeof(float);
-  if (smem > 48 * 1024) {
-    if (int status = allow_shared_memory<norm_rows_by_element<T>>(32768 * 4, "cudaFuncSetAttribute(layernorm_forward)"))
-      return status;
-  }
-  launch_dependent(norm_rows_by_element<T>, dim3((unsigned)p.rows), dim3(kElementThreads), (size_t)smem, stream, p);
-  return check_launch("layernorm_forward kernel launch");
+  if (p.hidden <= 128) return launch_by_element<T, 32, 8, 4, 0>(p, stream);
+  if (p.hidden <= 256) return launch_by_element<T, 32, 8, 8, 4>(p, stream);
+  if (p.hidden <= 512) return launch_by_element<T, 64, 4, 8, 4>(p, stream);
+  if (p.hidden <= 1024) return launch_by_element<T, 128, 2, 8, 4>(p, stream);
+  if (p.hidden <= 2048) return launch_by_element<T, 256, 1, 8, 4>(p, stream);
+  if (p.hidden <= 4096) return launch_by_element<T, 512, 1, 8, 4>(p, stream);
+  if (p.hidden <= 8192) return launch_by_element<T, 1024, 1, 8, 4>(p, stream);
+  if (p.hidden <= 16384) return launch_by_element<T, 1024, 1, 16, 8>(p, stream);
+  return launch_by_element<T, 1024, 1, 32, 16>(p, stream);
 }
 
 }  // namespace
