@@ -194,9 +194,9 @@ __device__ __forceinline__ void row_sums(float (&v)[COUNT], RowSums<LANES, COUNT
 }
 
 // ---- the rows of TENSORS matrices, copied ahead --------------------------------------------------------------------------
-// THREADS threads in groups of LANES; a group takes ROWS rows a turn (row, row + GROUPS, ...), and the next turns' bytes are
-// on their way to shared memory while it works on one.  Both forms give a thread the same columns of every row, as PAIRS
-// pairs, so it can keep what belongs to columns (sums over rows) in registers.  Bytes in flight per SM decide the depth:
+// THREADS threads in groups of LANES; a group walks its rows, and the next rows' bytes are on their way to shared memory
+// while it works on one.  Both forms give a thread the same columns of every row, as PAIRS pairs, so it can keep what
+// belongs to columns (weights, sums over rows) in registers.  Bytes in flight per SM decide the depth:
 // about 80 KB cover the latency of HBM3e at its bandwidth (44 B/ns per SM, 1 to 2 us under load).
 template <int STAGE_BYTES, int MOST_BYTES> constexpr int stages_for() {
   constexpr int wanted = 1 + (80 * 1024 + STAGE_BYTES - 1) / STAGE_BYTES, most = MOST_BYTES / STAGE_BYTES, within = wanted > 6 ? 6 : wanted < 3 ? 3 : wanted;
@@ -204,69 +204,65 @@ template <int STAGE_BYTES, int MOST_BYTES> constexpr int stages_for() {
   return within < most ? within : most;
 }
 
-// `wanted` rows a turn, or one where two stages of that many would not fit.
-constexpr int turn_rows(int wanted, int row_bytes, int most_bytes) { return wanted * row_bytes * 2 <= most_bytes ? wanted : 1; }
-
 // Rows of whole 16-byte vectors, 16-byte aligned.  Thread `lane` of a group owns the vectors lane, lane + LANES, ...; it
 // copies and reads them itself, so it waits for nothing but its own copies.
-template <typename T, int THREADS_, int LANES_, int VPT, int TENSORS, int ROWS_, int MOST_BYTES> struct VectorRows {
+template <typename T, int THREADS_, int LANES_, int VPT, int TENSORS, int MOST_BYTES> struct VectorRows {
   static constexpr int THREADS = THREADS_, LANES = LANES_, VEC = 16 / sizeof(T), PAIRS = VPT * VEC / 2, GROUPS = THREADS / LANES;
-  static constexpr int kSlot = THREADS * VPT * 16, ROWS = turn_rows(ROWS_, kSlot * TENSORS, MOST_BYTES), kStage = kSlot * TENSORS * ROWS, STAGES = stages_for<kStage, MOST_BYTES>(), kBytes = kStage * STAGES;
+  static constexpr int kSlot = THREADS * VPT * 16, kStage = kSlot * TENSORS, STAGES = stages_for<kStage, MOST_BYTES>(), kBytes = kStage * STAGES;
 
   unsigned char* shared;
   const T* tensors[TENSORS];
   size_t rows;
   int hidden, lane, stage;
 
-  __device__ __forceinline__ VectorRows(unsigned char* memory, const T* const (&sources)[TENSORS], size_t rows_, int hidden_, int lane_, int, int)
+  __device__ __forceinline__ VectorRows(unsigned char* memory, const T* const (&sources)[TENSORS], size_t rows_, int hidden_, int lane_, int)
       : shared(memory), rows(rows_), hidden(hidden_), lane(lane_), stage(0) {
 #pragma unroll
     for (int t = 0; t < TENSORS; ++t) tensors[t] = sources[t];
   }
-  __device__ __forceinline__ unsigned char* slot(int at, int r, int tensor, int j) const {
-    return shared + at * kStage + (r * TENSORS + tensor) * kSlot + (j * THREADS + threadIdx.x) * 16;
+  __device__ __forceinline__ unsigned char* slot(int at, int tensor, int j) const {
+    return shared + at * kStage + tensor * kSlot + (j * THREADS + threadIdx.x) * 16;
   }
   __device__ __forceinline__ int vector(int j) const { return lane + j * LANES; }
   __device__ __forceinline__ bool has(int j) const { return vector(j) * VEC < hidden; }
   __device__ __forceinline__ void fetch(size_t row, int at) {
+    if (row < rows) {
+      const size_t offset = row * (size_t)hidden;
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-      if (row + r * GROUPS < rows) {
-        const size_t offset = (row + r * GROUPS) * (size_t)hidden;
+      for (int j = 0; j < VPT; ++j) {
+        if (has(j)) {
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) {
-          if (has(j)) {
-#pragma unroll
-            for (int t = 0; t < TENSORS; ++t) copy_async_16(slot(at, r, t, j), tensors[t] + offset + vector(j) * VEC);
-          }
+          for (int t = 0; t < TENSORS; ++t) copy_async_16(slot(at, t, j), tensors[t] + offset + vector(j) * VEC);
         }
       }
     }
     copy_async_commit();
   }
-  __device__ __forceinline__ void start(size_t row, size_t stride) {
+  __device__ __forceinline__ void start(size_t row, size_t stride, int) {
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       if (!has(j)) {  // slots past the row's end are never copied to: zeros, so rows are read without a question
-        for (int at = 0; at < STAGES * ROWS * TENSORS; ++at)
+        for (int at = 0; at < STAGES * TENSORS; ++at)
           *reinterpret_cast<uint4*>(shared + at * kSlot + (j * THREADS + threadIdx.x) * 16) = make_uint4(0, 0, 0, 0);
       }
     }
 #pragma unroll
     for (int at = 0; at < STAGES - 1; ++at) fetch(row + at * stride, at);
   }
-  // The turn's rows have arrived, and later ones are on their way into the slots of the turn before it.
+  // The row has arrived, and a later one is on its way into the slots of the row before it.
   __device__ __forceinline__ void arrive(size_t row, size_t stride) {
     fetch(row + (STAGES - 1) * stride, stage == 0 ? STAGES - 1 : stage - 1);
     copy_async_wait<STAGES - 1>();
   }
+  __device__ __forceinline__ void before_sums() {}
+  __device__ __forceinline__ void after_sums(size_t, size_t) {}
   __device__ __forceinline__ void next() { stage = stage + 1 == STAGES ? 0 : stage + 1; }
 
-  // Pairs of one tensor's row; zeros past the row's end.
-  __device__ __forceinline__ void get(int r, int tensor, F2 (&out)[PAIRS]) const {
+  // The row's pairs of one tensor; zeros past the row's end.
+  __device__ __forceinline__ void get(int tensor, F2 (&out)[PAIRS]) const {
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-      const Pack<T, VEC> v = *reinterpret_cast<const Pack<T, VEC>*>(slot(stage, r, tensor, j));
+      const Pack<T, VEC> v = *reinterpret_cast<const Pack<T, VEC>*>(slot(stage, tensor, j));
 #pragma unroll
       for (int i = 0; i < VEC / 2; ++i) out[j * (VEC / 2) + i] = Pairs<T>::get(v, i);
     }
@@ -289,68 +285,76 @@ template <typename T, int THREADS_, int LANES_, int VPT, int TENSORS, int ROWS_,
 
 // Rows of any width in tensors whose first element is 16-byte aligned: the group copies the 16-byte windows that cover the
 // row (the last one of a tensor only as far as the tensor goes), and thread `lane` owns the columns lane, lane + LANES, ...
-// The copies are other threads' too, so the group meets at its barrier before it reads a row.  SURE: so many of a thread's
-// columns lie inside every row that this form is used for (LANES * SURE <= hidden), and are not asked about.
-template <typename T, int THREADS_, int LANES_, int COLUMNS, int SURE, int TENSORS, int ROWS_, int MOST_BYTES> struct ShiftedRows {
+// The copies are other threads' too.  One barrier a row does for that: a thread waits for its copies of the next row before
+// it meets the others at the barrier of the row's (first) sums, and copies into the slots of the row before after it.
+// SURE: so many of a thread's columns lie inside every row that this form is used for (LANES * SURE <= hidden), and are
+// not asked about.
+template <typename T, int THREADS_, int LANES_, int COLUMNS, int SURE, int TENSORS, int MOST_BYTES> struct ShiftedRows {
   static constexpr int THREADS = THREADS_, LANES = LANES_, PAIRS = COLUMNS / 2, GROUPS = THREADS / LANES;
-  static constexpr int kSlot = LANES * COLUMNS * (int)sizeof(T) + 32, ROWS = turn_rows(ROWS_, kSlot * TENSORS * GROUPS, MOST_BYTES), kGroup = kSlot * TENSORS * ROWS, kStage = kGroup * GROUPS,
-                       STAGES = stages_for<kStage, MOST_BYTES>(), kBytes = kStage * STAGES;
+  static constexpr int kSlot = LANES * COLUMNS * (int)sizeof(T) + 32, kGroup = kSlot * TENSORS, kStage = kGroup * GROUPS,
+                       STAGES = stages_for<kStage, MOST_BYTES>(), kBytes = kStage * STAGES, kWindows = COLUMNS * (int)sizeof(T) / 16 + 1;
+  static_assert(STAGES >= 3, "the next row's copies are waited for a row ahead");
 
   unsigned char* shared;
-  const T* tensors[TENSORS];
-  size_t rows, row_at_hand;
-  int hidden, lane, barrier, stage;
+  const unsigned char* tensors[TENSORS];
+  size_t rows;
+  int hidden, lane, stage;
+  uint32_t shift;  // bytes from the window's start to the row's, of the row at hand
 
-  __device__ __forceinline__ ShiftedRows(unsigned char* memory, const T* const (&sources)[TENSORS], size_t rows_, int hidden_, int lane_, int group,
-                                         int barrier_)
-      : shared(memory + group * kGroup), rows(rows_), row_at_hand(0), hidden(hidden_), lane(lane_), barrier(barrier_), stage(0) {
+  __device__ __forceinline__ ShiftedRows(unsigned char* memory, const T* const (&sources)[TENSORS], size_t rows_, int hidden_, int lane_, int group)
+      : shared(memory + group * kGroup), rows(rows_), hidden(hidden_), lane(lane_), stage(0), shift(0) {
 #pragma unroll
-    for (int t = 0; t < TENSORS; ++t) tensors[t] = sources[t];
+    for (int t = 0; t < TENSORS; ++t) tensors[t] = reinterpret_cast<const unsigned char*>(sources[t]);
   }
-  __device__ __forceinline__ unsigned char* slot(int at, int r, int tensor) const { return shared + at * kStage + (r * TENSORS + tensor) * kSlot; }
   __device__ __forceinline__ void fetch(size_t row, int at) {
+    if (row < rows) {
+      const uint32_t row_bytes = (uint32_t)hidden * (uint32_t)sizeof(T);
+      const size_t begin = row * row_bytes;
+      const uint32_t inside = (uint32_t)begin & 15u, bytes = inside + row_bytes, windows = (bytes + 15) / 16;
+      const size_t window_end = begin - inside + windows * 16u, end = rows * row_bytes;
+      const uint32_t tail = window_end > end ? 16u - (uint32_t)(window_end - end) : 16u;  // of the last window, nothing behind the tensor
+      const size_t from = begin - inside + (size_t)lane * 16;
+      unsigned char* to = shared + at * kStage + lane * 16;
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-      if (row + r * GROUPS < rows) {
-        const size_t begin = (row + r * GROUPS) * (size_t)hidden * sizeof(T), window = begin & ~(size_t)15, end = rows * (size_t)hidden * sizeof(T);
-        const int vectors = (int)((begin - window + (size_t)hidden * sizeof(T) + 15) / 16);
-        for (int v = lane; v < vectors; v += LANES) {
-          const size_t from = window + (size_t)v * 16;
-          const uint32_t bytes = end - from < 16 ? (uint32_t)(end - from) : 16;
+      for (int w = 0; w < kWindows; ++w) {
+        const uint32_t v = lane + w * LANES;
+        if (v < windows) {
+          const uint32_t size = v + 1 == windows ? tail : 16u;
 #pragma unroll
-          for (int t = 0; t < TENSORS; ++t) copy_async_part(slot(at, r, t) + v * 16, reinterpret_cast<const unsigned char*>(tensors[t]) + from, bytes);
+          for (int t = 0; t < TENSORS; ++t) copy_async_part(to + t * kSlot + w * (LANES * 16), tensors[t] + from + w * (LANES * 16), size);
         }
       }
     }
     copy_async_commit();
   }
-  __device__ __forceinline__ void start(size_t row, size_t stride) {
+  __device__ __forceinline__ void start(size_t row, size_t stride, int barrier) {
 #pragma unroll
     for (int at = 0; at < STAGES - 1; ++at) fetch(row + at * stride, at);
-  }
-  __device__ __forceinline__ void arrive(size_t row, size_t stride) {
     copy_async_wait<STAGES - 2>();
-    row_barrier<LANES>(barrier);  // everyone's copies have landed, and everyone is done with the turn before
-    fetch(row + (STAGES - 1) * stride, stage == 0 ? STAGES - 1 : stage - 1);
-    row_at_hand = row;
+    row_barrier<LANES>(barrier);
   }
+  __device__ __forceinline__ void arrive(size_t row, size_t) { shift = (uint32_t)(row * ((uint32_t)hidden * (uint32_t)sizeof(T))) & 15u; }
+  __device__ __forceinline__ void before_sums() {
+    copy_async_wait<STAGES - 3>();
+    if constexpr (LANES <= 32) __syncwarp();  // otherwise the sums' own barrier
+  }
+  __device__ __forceinline__ void after_sums(size_t row, size_t stride) { fetch(row + (STAGES - 1) * stride, stage == 0 ? STAGES - 1 : stage - 1); }
   __device__ __forceinline__ void next() { stage = stage + 1 == STAGES ? 0 : stage + 1; }
 
-  __device__ __forceinline__ void get(int r, int tensor, F2 (&out)[PAIRS]) const {
-    const int shift = (int)(((row_at_hand + r * GROUPS) * (size_t)hidden * sizeof(T)) & 15);
-    const T* row = reinterpret_cast<const T*>(slot(stage, r, tensor) + shift);
+  __device__ __forceinline__ void get(int tensor, F2 (&out)[PAIRS]) const {
+    const T* row = reinterpret_cast<const T*>(shared + stage * kStage + tensor * kSlot + shift) + lane;
 #pragma unroll
-    for (int i = 0; i < PAIRS; ++i) {
-      out[i] = make_f2(has(2 * i) ? Conv<float, T>::widen(row[column(i, 0)]) : 0.0f, has(2 * i + 1) ? Conv<float, T>::widen(row[column(i, 1)]) : 0.0f);
-    }
+    for (int i = 0; i < PAIRS; ++i)
+      out[i] = make_f2(has(2 * i) ? Conv<float, T>::widen(row[2 * i * LANES]) : 0.0f, has(2 * i + 1) ? Conv<float, T>::widen(row[(2 * i + 1) * LANES]) : 0.0f);
   }
   __device__ __forceinline__ void put(T* row, const F2 (&in)[PAIRS]) const {
+    row += lane;
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) {
-      float low, high;
-      split(in[i], low, high);
-      if (has(2 * i)) row[column(i, 0)] = Conv<float, T>::narrow(low);
-      if (has(2 * i + 1)) row[column(i, 1)] = Conv<float, T>::narrow(high);
+      Pack<T, 2> v;  // rounded in pairs: one instruction
+      Pairs<T>::set(v, 0, in[i]);
+      if (has(2 * i)) row[2 * i * LANES] = v.v[0];
+      if (has(2 * i + 1)) row[(2 * i + 1) * LANES] = v.v[1];
     }
   }
   __device__ __forceinline__ int column(int pair, int half) const { return lane + (2 * pair + half) * LANES; }

@@ -45,10 +45,10 @@ norm_backward_rows(const __grid_constant__ Backward<T> p) {
   sources[0] = p.grad_out;
   sources[1] = p.x;
   if constexpr (RESIDUAL) sources[2] = p.grad_resid;
-  Rows rows(shared, sources, p.rows, p.hidden, lane, group, barrier);
+  Rows rows(shared, sources, p.rows, p.hidden, lane, group);
   const size_t stride = (size_t)gridDim.x * GROUPS;
   size_t row = (size_t)blockIdx.x * GROUPS + group;
-  rows.start(row, stride);
+  rows.start(row, stride, barrier);
   F2 weight[PAIRS], grad_weight[PAIRS], grad_bias[PAIRS];
   column_pairs<T>(rows, p.weight, p.wide, weight);
 #pragma unroll
@@ -66,8 +66,8 @@ norm_backward_rows(const __grid_constant__ Backward<T> p) {
     F2 sum_g = both(0.0f), sum_gn = both(0.0f);
     const F2 factor = both(rstd);
     if (active) {
-      rows.get(0, 0, g);
-      rows.get(0, 1, n);
+      rows.get(0, g);
+      rows.get(1, n);
       const F2 minus_mean = both(-mean);
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {
@@ -80,13 +80,15 @@ norm_backward_rows(const __grid_constant__ Backward<T> p) {
       }
     }
     float sums[2] = {total(sum_g), total(sum_gn)};
+    rows.before_sums();
     row_sums<LANES>(sums, &scratch[group], turn, barrier);
+    rows.after_sums(row, stride);
     if (active) {
       const F2 minus_mean_g = both(-sums[0] * scale), minus_mean_gn = both(-sums[1] * scale);
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) g[i] = fma2(n[i], minus_mean_gn, g[i] + minus_mean_g);
       if constexpr (RESIDUAL) {
-        rows.get(0, 2, n);
+        rows.get(2, n);
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) g[i] = fma2(g[i], factor, n[i]);
       } else {
@@ -99,8 +101,8 @@ norm_backward_rows(const __grid_constant__ Backward<T> p) {
     rstd = next_rstd;
   }
   copy_async_wait<0>();
-  // the CTA's share of the column sums: groups inside a warp join by exchanges, then warps (or groups) add up in shared
-  // memory, one after the other
+  // the CTA's share of the column sums: groups inside a warp join by exchanges, warps (or groups) lay theirs out beside each
+  // other in shared memory, over row slots that nobody reads any more, and every thread adds up some columns
   if constexpr (LANES < 32) {
 #pragma unroll
     for (int offset = LANES; offset < 32; offset <<= 1) {
@@ -120,30 +122,36 @@ norm_backward_rows(const __grid_constant__ Backward<T> p) {
   }
   constexpr int SET = LANES < 32 ? 32 : LANES, SETS = kRowThreads / SET;
   constexpr bool STAGED = SETS > 1 || CLUSTER;
+  static_assert(!STAGED || Rows::kBytes >= SETS * LANES * PAIRS * 2 * 2 * (int)sizeof(float), "the sets have to fit");
   float* share = p.partial + (size_t)blockIdx.x * 2 * p.hidden;
-  float* columns = STAGED ? reinterpret_cast<float*>(shared) : share;  // [2][hidden], over row slots that nobody reads any more
-  for (int set = 0; set < SETS; ++set) {
-    __syncthreads();
-    if ((int)threadIdx.x / SET == set && (threadIdx.x & 31) % SET < LANES) {
+  float* columns = STAGED ? reinterpret_cast<float*>(shared) : share;  // [sets][2][hidden]
+  if constexpr (STAGED) __syncthreads();
+  if ((threadIdx.x & 31) % SET < LANES) {
+    float* mine = columns + (threadIdx.x / SET) * 2 * p.hidden;
 #pragma unroll
-      for (int i = 0; i < PAIRS; ++i) {
-        float w[2], b[2];
-        split(grad_weight[i], w[0], w[1]);
-        split(grad_bias[i], b[0], b[1]);
+    for (int i = 0; i < PAIRS; ++i) {
+      float w[2], b[2];
+      split(grad_weight[i], w[0], w[1]);
+      split(grad_bias[i], b[0], b[1]);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int c = rows.column(i, half);
-          if (c < p.hidden) {
-            columns[c] = set ? columns[c] + w[half] : w[half];
-            columns[p.hidden + c] = set ? columns[p.hidden + c] + b[half] : b[half];
-          }
+      for (int half = 0; half < 2; ++half) {
+        const int c = rows.column(i, half);
+        if (c < p.hidden) {
+          mine[c] = w[half];
+          mine[p.hidden + c] = b[half];
         }
       }
     }
   }
-  if constexpr (STAGED) __syncthreads();
-  if constexpr (STAGED && !CLUSTER) {
-    for (int c = threadIdx.x; c < 2 * p.hidden; c += kRowThreads) share[c] = columns[c];
+  if constexpr (STAGED) {
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * p.hidden; c += kRowThreads) {
+      float sum = columns[c];
+#pragma unroll
+      for (int set = 1; set < SETS; ++set) sum += columns[set * 2 * p.hidden + c];
+      (CLUSTER ? columns : share)[c] = sum;
+    }
+    if constexpr (CLUSTER) __syncthreads();
   }
   if constexpr (CLUSTER) {
     cluster_barrier();
@@ -299,8 +307,8 @@ template <typename T> int backward(Backward<T> p, bool aligned, cudaStream_t str
     // two vectors a thread (16 columns, 8 for f32): weight, both column sums and the row's two products fit the registers
 #define BB200_VECTOR_ROWS(LANES, VPT)                                                                                  \
   if (nvec <= (LANES) * (VPT))                                                                                         \
-    return p.grad_resid ? launch_rows<T, VectorRows<T, kRowThreads, LANES, VPT, 3, 1, kMostSmem>, true, true>(p, stream)        \
-                        : launch_rows<T, VectorRows<T, kRowThreads, LANES, VPT, 2, 1, kMostSmem>, false, true>(p, stream)
+    return p.grad_resid ? launch_rows<T, VectorRows<T, kRowThreads, LANES, VPT, 3, kMostSmem>, true, true>(p, stream)        \
+                        : launch_rows<T, VectorRows<T, kRowThreads, LANES, VPT, 2, kMostSmem>, false, true>(p, stream)
     BB200_VECTOR_ROWS(4, 2);
     BB200_VECTOR_ROWS(8, 2);
     BB200_VECTOR_ROWS(16, 2);
@@ -314,15 +322,16 @@ template <typename T> int backward(Backward<T> p, bool aligned, cudaStream_t str
   } else if (aligned) {
 #define BB200_SHIFTED_ROWS(LANES, COLUMNS, SURE)                                                                           \
   if (p.hidden <= (LANES) * (COLUMNS))                                                                                 \
-    return p.grad_resid ? launch_rows<T, ShiftedRows<T, kRowThreads, LANES, COLUMNS, SURE, 3, 1, kMostSmem>, true, false>(p, stream)   \
-                        : launch_rows<T, ShiftedRows<T, kRowThreads, LANES, COLUMNS, SURE, 2, 1, kMostSmem>, false, false>(p, stream)
+    return p.grad_resid ? launch_rows<T, ShiftedRows<T, kRowThreads, LANES, COLUMNS, SURE, 3, kMostSmem>, true, false>(p, stream)   \
+                        : launch_rows<T, ShiftedRows<T, kRowThreads, LANES, COLUMNS, SURE, 2, kMostSmem>, false, false>(p, stream)
+    constexpr int kColumns = 2 * VEC;  // 16, or 8 of f32, so that three stages fit
     BB200_SHIFTED_ROWS(32, 4, 0);
     BB200_SHIFTED_ROWS(32, 8, 4);
-    BB200_SHIFTED_ROWS(32, 16, 8);
-    BB200_SHIFTED_ROWS(64, 16, 8);
-    BB200_SHIFTED_ROWS(128, 16, 8);
-    BB200_SHIFTED_ROWS(256, 16, 8);
-    BB200_SHIFTED_ROWS(512, 16, 8);
+    if constexpr (VEC == 8) BB200_SHIFTED_ROWS(32, 16, 8);
+    BB200_SHIFTED_ROWS(64, kColumns, kColumns / 2);
+    BB200_SHIFTED_ROWS(128, kColumns, kColumns / 2);
+    BB200_SHIFTED_ROWS(256, kColumns, kColumns / 2);
+    BB200_SHIFTED_ROWS(512, kColumns, kColumns / 2);
 #undef BB200_SHIFTED_ROWS
   }
   const size_t blocks = (p.hidden + kElementThreads - 1) / kElementThreads;

@@ -40,10 +40,10 @@ norm_rows(const __grid_constant__ Forward<T> p) {
   const T* sources[RESIDUAL ? 2 : 1];
   sources[0] = p.x;
   if constexpr (RESIDUAL) sources[1] = p.residual;
-  Rows rows(shared, sources, p.rows, p.hidden, lane, group, barrier);
+  Rows rows(shared, sources, p.rows, p.hidden, lane, group);
   const size_t stride = (size_t)gridDim.x * GROUPS;
   size_t row = (size_t)blockIdx.x * GROUPS + group;
-  rows.start(row, stride);
+  rows.start(row, stride, barrier);
   F2 weight[PAIRS], bias[PAIRS];
   column_pairs<T>(rows, p.weight, p.wide, weight);
   column_pairs<T>(rows, p.bias, p.wide, bias);
@@ -57,10 +57,10 @@ norm_rows(const __grid_constant__ Forward<T> p) {
     F2 sum2 = both(0.0f);
     const size_t offset = row * (size_t)p.hidden;
     if (active) {
-      rows.get(0, 0, s);
+      rows.get(0, s);
       if constexpr (RESIDUAL) {
         F2 r[PAIRS];
-        rows.get(0, 1, r);
+        rows.get(1, r);
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) s[i] = s[i] + r[i];
         rows.put(p.out_resid + offset, s);
@@ -69,7 +69,9 @@ norm_rows(const __grid_constant__ Forward<T> p) {
       for (int i = 0; i < PAIRS; ++i) sum2 = sum2 + s[i];
     }
     float sum[1] = {total(sum2)};
+    rows.before_sums();
     row_sums<LANES>(sum, &scratch[group], turn, barrier);
+    rows.after_sums(row, stride);
     const float mean = sum[0] * scale;
     F2 centred = both(0.0f);
     if (active) {
@@ -359,7 +361,7 @@ template <typename T> int forward(const Forward<T>& p, bool aligned, cudaStream_
     // other's sums (8192 wide, bf16: 395 us against 523 us for one group of 512).
 #define BB200_VECTOR_ROWS(LANES, VPT)                                                              \
   if (nvec <= (LANES) * (VPT))                                                                     \
-    return p.residual ? launch_rows<T, VectorRows<T, kRowThreads, LANES, VPT, 2, 1, kMostSmem>, true>(p, stream) : launch_rows<T, VectorRows<T, kRowThreads, LANES, VPT, 1, 1, kMostSmem>, false>(p, stream)
+    return p.residual ? launch_rows<T, VectorRows<T, kRowThreads, LANES, VPT, 2, kMostSmem>, true>(p, stream) : launch_rows<T, VectorRows<T, kRowThreads, LANES, VPT, 1, kMostSmem>, false>(p, stream)
     BB200_VECTOR_ROWS(4, 2);
     BB200_VECTOR_ROWS(8, 2);
     BB200_VECTOR_ROWS(16, 2);
@@ -380,12 +382,13 @@ template <typename T> int forward(const Forward<T>& p, bool aligned, cudaStream_
   if (aligned && p.hidden > 256 && p.rows * (size_t)p.hidden > ((size_t)1 << 24)) {
 #define BB200_SHIFTED_ROWS(LANES, COLUMNS, SURE)                                                    \
   if (p.hidden <= (LANES) * (COLUMNS))                                                             \
-    return p.residual ? launch_rows<T, ShiftedRows<T, kRowThreads, LANES, COLUMNS, SURE, 2, 1, kMostSmem>, true>(p, stream) : launch_rows<T, ShiftedRows<T, kRowThreads, LANES, COLUMNS, SURE, 1, 1, kMostSmem>, false>(p, stream)
-    BB200_SHIFTED_ROWS(32, 16, 8);
-    BB200_SHIFTED_ROWS(64, 16, 8);
-    BB200_SHIFTED_ROWS(128, 16, 8);
-    BB200_SHIFTED_ROWS(256, 16, 8);
-    BB200_SHIFTED_ROWS(512, 16, 8);
+    return p.residual ? launch_rows<T, ShiftedRows<T, kRowThreads, LANES, COLUMNS, SURE, 2, kMostSmem>, true>(p, stream) : launch_rows<T, ShiftedRows<T, kRowThreads, LANES, COLUMNS, SURE, 1, kMostSmem>, false>(p, stream)
+    constexpr int kColumns = 2 * VEC;
+    if constexpr (VEC == 8) BB200_SHIFTED_ROWS(32, kColumns, kColumns / 2);
+    BB200_SHIFTED_ROWS(64, kColumns, kColumns / 2);
+    BB200_SHIFTED_ROWS(128, kColumns, kColumns / 2);
+    BB200_SHIFTED_ROWS(256, kColumns, kColumns / 2);
+    BB200_SHIFTED_ROWS(512, kColumns, kColumns / 2);
 #undef BB200_SHIFTED_ROWS
   }
   if (p.hidden <= 128) return launch_by_element<T, 32, 8, 4, 0>(p, stream);
