@@ -225,7 +225,9 @@ struct SortedList {
 
 // Up to 65536 tokens in one launch: one cluster of up to 16 CTAs holds them all in shared memory.  Every pass ranks in
 // each CTA, adds up the CTAs' digit counts through distributed shared memory and sends every element to its place there;
-// nobody touches another CTA's memory after the last pass's barrier.
+// nobody touches another CTA's memory after the last pass's barrier.  A sort keeps few SMs busy, so where the whole table is
+// written the launch has more clusters, which meanwhile fill the table's first rows with zeros (the sums overwrite those
+// that tokens name).
 constexpr uint32_t kMostCtas = 16;
 
 template <int R> struct ClusterSort {
@@ -239,11 +241,16 @@ template <int R> struct ClusterSort {
 template <typename Id, int R>
 __global__ void __launch_bounds__(kSortThreads, 1)
 sort_in_cluster(const Id* __restrict__ tokens, uint32_t count, uint32_t vocabulary, long long padding, int passes, int digit_bits, uint32_t ctas,
-                const __grid_constant__ SortedList list, uint8_t* __restrict__ named, int* status_word) {
+                const __grid_constant__ SortedList list, uint8_t* __restrict__ named, uint4* __restrict__ zeros, size_t zero_vectors, int* status_word) {
   constexpr uint32_t kEach = kSortThreads * R;
   extern __shared__ __align__(16) unsigned char shared[];
   ClusterSort<R>& s = *reinterpret_cast<ClusterSort<R>*>(shared);
   dependent_launch_prologue();
+  if (blockIdx.x >= ctas) {  // the other clusters
+    const size_t stride = (size_t)(gridDim.x - ctas) * kSortThreads;
+    for (size_t i = (size_t)(blockIdx.x - ctas) * kSortThreads + threadIdx.x; i < zero_vectors; i += stride) __stcs(zeros + i, make_uint4(0, 0, 0, 0));
+    return;
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank_of_cta = cluster_rank();
   uint32_t key[R], position[R];
@@ -391,6 +398,7 @@ struct Segments {
   uint32_t* crossings;
   float* partial;  // [chunks][2][hidden]: the sums of a chunk's first run (it began before) and of its last (it goes on)
   uint32_t count, vocabulary, chunk_length, chunks;
+  uint32_t fill_from;  // the first row that may still need zeros
   int steps, lane_bits;
   bool wide;  // table and gradient are aligned to 32 bytes
 };
@@ -481,7 +489,7 @@ join_and_fill(const __grid_constant__ Segments s, W* __restrict__ grad_table, fl
   const size_t hidden = (size_t)s.steps * VEC;
   if (blockIdx.x >= join_blocks) {
     const int lanes = 1 << s.lane_bits, groups = kThreads >> s.lane_bits;
-    const size_t first = (size_t)(blockIdx.x - join_blocks) * groups * kFillRows + (threadIdx.x >> s.lane_bits);
+    const size_t first = s.fill_from + (size_t)(blockIdx.x - join_blocks) * groups * kFillRows + (threadIdx.x >> s.lane_bits);
     bool empty[kFillRows];
 #pragma unroll
     for (int r = 0; r < kFillRows; ++r) empty[r] = first + r * groups < s.vocabulary && !named[first + r * groups];
@@ -545,23 +553,26 @@ struct GradientCall {
 inline size_t round_up(size_t n) { return (n + 255) & ~(size_t)255; }
 
 template <typename Id, int R>
-int launch_cluster_sort(const GradientCall& call, unsigned ctas, int passes, int digit_bits, const SortedList& list, uint8_t* named, cudaStream_t stream) {
+int launch_cluster_sort(const GradientCall& call, unsigned ctas, int passes, int digit_bits, const SortedList& list, uint8_t* named, size_t zero_bytes,
+                        cudaStream_t stream) {
+  const unsigned fill = zero_bytes ? ((unsigned)multiprocessor_count() + ctas - 1) / ctas * ctas : 0;  // whole clusters
   if (ctas > 8) {  // beyond the portable size; the attribute is cheap to set again
     if (int status = check_runtime(cudaFuncSetAttribute(sort_in_cluster<Id, R>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
                                    "cudaFuncSetAttribute(embedding_backward sort)"))
       return status;
   }
   if (int status = allow_shared_memory<sort_in_cluster<Id, R>>((int)sizeof(ClusterSort<R>), "cudaFuncSetAttribute(embedding_backward sort)")) return status;
-  launch_dependent_cluster(sort_in_cluster<Id, R>, dim3(ctas), dim3(kSortThreads), ctas, sizeof(ClusterSort<R>), stream,
+  launch_dependent_cluster(sort_in_cluster<Id, R>, dim3(ctas + fill), dim3(kSortThreads), ctas, sizeof(ClusterSort<R>), stream,
                            static_cast<const Id*>(call.tokens), (uint32_t)call.count, (uint32_t)call.vocabulary, call.padding, passes, digit_bits,
-                           (uint32_t)ctas, list, named, device_status_word());
+                           (uint32_t)ctas, list, named, static_cast<uint4*>(call.grad_table), zero_bytes / 16, device_status_word());
   return check_launch("embedding_backward sort launch");
 }
 
 // Sorts the call's tokens into `list`.  `spare`: as much again, for the passes between, and `counts`, where there are more
 // than one cluster holds.
 template <typename Id>
-int sort_tokens(const GradientCall& call, const SortedList& list, const SortedList& spare, uint32_t* counts, uint8_t* named, cudaStream_t stream) {
+int sort_tokens(const GradientCall& call, const SortedList& list, const SortedList& spare, uint32_t* counts, uint8_t* named, size_t zero_bytes,
+                cudaStream_t stream) {
   const uint32_t count = (uint32_t)call.count, vocabulary = (uint32_t)call.vocabulary;
   int bits = 1;  // of the keys 0 .. vocabulary
   while (((unsigned long long)call.vocabulary >> bits) != 0) ++bits;
@@ -572,9 +583,9 @@ int sort_tokens(const GradientCall& call, const SortedList& list, const SortedLi
     return n;
   };
   // Few elements a thread and many CTAs: 65536 tokens 24 us with 16 CTAs, 35 us with eight of twice the elements.
-  if (count <= 16384) return launch_cluster_sort<Id, 1>(call, ctas(1024), passes, digit_bits, list, named, stream);
-  if (count <= 32768) return launch_cluster_sort<Id, 2>(call, ctas(2048), passes, digit_bits, list, named, stream);
-  if (count <= 65536) return launch_cluster_sort<Id, 4>(call, ctas(4096), passes, digit_bits, list, named, stream);
+  if (count <= 16384) return launch_cluster_sort<Id, 1>(call, ctas(1024), passes, digit_bits, list, named, zero_bytes, stream);
+  if (count <= 32768) return launch_cluster_sort<Id, 2>(call, ctas(2048), passes, digit_bits, list, named, zero_bytes, stream);
+  if (count <= 65536) return launch_cluster_sort<Id, 4>(call, ctas(4096), passes, digit_bits, list, named, zero_bytes, stream);
   const Id* tokens = static_cast<const Id*>(call.tokens);
   const int tiles = (int)((call.count + kTile - 1) / kTile);
   const uint32_t mask = (1u << digit_bits) - 1;
@@ -645,9 +656,18 @@ template <typename G, typename W, int VEC, bool ADD> int gradient(const Gradient
   if (named) {
     if (int status = check_runtime(cudaMemsetAsync(named, 0, call.vocabulary, stream), "cudaMemsetAsync(embedding_backward)")) return status;
   }
-  if (int status = wide_tokens ? sort_tokens<int64_t>(call, sorted, other, counts, named, stream)
-                               : sort_tokens<int32_t>(call, sorted, other, counts, named, stream))
+  // Rows that are filled with zeros during the sort: whole sixteens, for about as many bytes as the idle SMs write meanwhile
+  // (65536 tokens take 24 us); the rows from there on are filled behind the sums.
+  size_t early_rows = 0;
+  if (named && !spare && aligned16(call.grad_table)) {
+    const size_t most = count * 1536 / (call.hidden * sizeof(W)) / 16 * 16, all = call.vocabulary / 16 * 16;
+    early_rows = most < all ? most : all;
+  }
+  const size_t zero_bytes = early_rows * call.hidden * sizeof(W);
+  if (int status = wide_tokens ? sort_tokens<int64_t>(call, sorted, other, counts, named, zero_bytes, stream)
+                               : sort_tokens<int32_t>(call, sorted, other, counts, named, zero_bytes, stream))
     return status;
+  s.fill_from = (uint32_t)early_rows;
   s.keys = sorted.keys;
   s.order = sorted.order;
   s.crossings = sorted.crossings;
@@ -659,7 +679,7 @@ template <typename G, typename W, int VEC, bool ADD> int gradient(const Gradient
   // at most one run crosses each border between two chunks
   const size_t most_items = (size_t)(s.chunks - 1) * ((steps + 31) / 32), join_most = (size_t)multiprocessor_count() * 8;
   const unsigned join_blocks = (unsigned)(most_items < join_most ? most_items : join_most);
-  const unsigned fill_blocks = named ? (unsigned)((call.vocabulary + groups * kFillRows - 1) / (groups * kFillRows)) : 0;
+  const unsigned fill_blocks = named ? (unsigned)((call.vocabulary - early_rows + groups * kFillRows - 1) / (groups * kFillRows)) : 0;
   if (join_blocks + fill_blocks > 0) {
     launch_dependent(join_and_fill<W, VEC, ADD>, dim3(join_blocks + fill_blocks), dim3(kThreads), 0, stream, s, table, call.scale, join_blocks,
                      static_cast<const uint8_t*>(named));
