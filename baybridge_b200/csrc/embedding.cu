@@ -220,7 +220,7 @@ __device__ __forceinline__ uint32_t exclusive_over_bins(uint32_t value, uint32_t
 struct SortedList {
   uint32_t* keys;
   uint32_t* order;
-  uint32_t* crossings;  // [0]: how many runs cross a chunk's border (set to 0 here), then their first chunks
+  uint32_t* crossings;  // see Segments; the two counts are set to 0 here
 };
 
 // Up to 65536 tokens in one launch: one cluster of up to 16 CTAs holds them all in shared memory.  Every pass ranks in
@@ -261,7 +261,7 @@ sort_in_cluster(const Id* __restrict__ tokens, uint32_t count, uint32_t vocabula
     key[r] = position[r] < count ? key_of(tokens[position[r]], vocabulary, padding, status_word) : vocabulary;
     if (named && key[r] < vocabulary) named[key[r]] = 1;
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) list.crossings[0] = 0;
+  if (blockIdx.x == 0 && threadIdx.x < 2) list.crossings[threadIdx.x] = 0;
   for (int pass = 0; pass < passes; ++pass) {
     uint32_t digit[R], rank[R];
 #pragma unroll
@@ -388,13 +388,17 @@ scatter_digits(const Id* __restrict__ tokens, const uint32_t* __restrict__ keys,
       list.order[to] = position[r];
     }
   }
-  if (last && blockIdx.x == 0 && threadIdx.x == 0) list.crossings[0] = 0;
+  if (last && blockIdx.x == 0 && threadIdx.x < 2) list.crossings[threadIdx.x] = 0;
 }
 
 // ---- segmented sums ---------------------------------------------------------------------------------------------------
+constexpr uint32_t kShortSpan = 8;
+
 struct Segments {
   const uint32_t* keys;   // sorted tokens
   const uint32_t* order;  // their positions
+  // the runs that cross a chunk's border, by the chunk where they begin: [0] how many reach into fewer than kShortSpan further
+  // chunks, [1] how many into more, then room for all of them, the short ones from the front and the long ones from the back
   uint32_t* crossings;
   float* partial;  // [chunks][2][hidden]: the sums of a chunk's first run (it began before) and of its last (it goes on)
   uint32_t count, vocabulary, chunk_length, chunks;
@@ -471,14 +475,20 @@ sum_chunks(const __grid_constant__ Segments s, const G* __restrict__ grad_out, W
     }
     if (open) {
       store_stream_32<float, VEC>(s.partial + (chunk * 2 + (began_before ? 0 : 1)) * hidden + column, sum.values(), true);
-      if (!began_before && step == 0) s.crossings[1 + atomicAdd(s.crossings, 1u)] = (uint32_t)chunk;
+      if (!began_before && step == 0) {
+        const size_t probe = chunk + kShortSpan;
+        const bool is_long = probe < s.chunks && s.keys[probe * s.chunk_length] == keys[s.chunk_length - 1];
+        const uint32_t at = atomicAdd(s.crossings + is_long, 1u);
+        s.crossings[is_long ? 1 + s.chunks - at : 2 + at] = (uint32_t)chunk;
+      }
     }
   }
 }
 
-// Two jobs in one launch.  The first `join_blocks` CTAs join the partial sums of the runs that cross a chunk's border: 32
-// vector columns of one run at a time, eight warps over its chunks, added up in a fixed order.  The other CTAs, where the
-// whole table is written, fill the rows that no token names with zeros; the joins hide behind them.
+// Two jobs in one launch.  The first `join_blocks` CTAs join the partial sums of the runs that cross a chunk's border, 32
+// vector columns of one run at a time and in a fixed order: a warp for a run of a few chunks, the CTA's eight warps over the
+// chunks of a long one.  The other CTAs, where the whole table is written, fill the rows that no token names with zeros; the
+// joins hide behind them.
 constexpr int kFillRows = 4;  // rows that a group looks at together
 
 template <typename W, int VEC, bool ADD>
@@ -507,9 +517,27 @@ join_and_fill(const __grid_constant__ Segments s, W* __restrict__ grad_table, fl
   }
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const uint32_t tiles = (uint32_t)(s.steps + 31) / 32;
-  const unsigned long long items = (unsigned long long)s.crossings[0] * tiles;
+  const unsigned long long short_items = (unsigned long long)s.crossings[0] * tiles, items = (unsigned long long)s.crossings[1] * tiles;
+  for (unsigned long long item = (unsigned long long)blockIdx.x * (kThreads / 32) + slice; item < short_items; item += (unsigned long long)join_blocks * (kThreads / 32)) {
+    const size_t chunk = s.crossings[2 + item / tiles], probe = chunk + 1 + lane;
+    const int step = (int)(item % tiles) * 32 + lane;
+    const uint32_t key = s.keys[(chunk + 1) * s.chunk_length - 1];
+    const int further = __popc(__ballot_sync(0xffffffffu, probe < s.chunks && s.keys[probe * s.chunk_length] == key));
+    if (step < s.steps) {
+      const float* from = s.partial + (chunk * 2 + 1) * hidden + (size_t)step * VEC;
+      Sum<VEC> sum;
+      sum.clear();
+      sum.add(load_stream_32<float, VEC>(from, true));
+      from += hidden;
+#pragma unroll 4
+      for (int c = 0; c < further; ++c) sum.add(load_stream_32<float, VEC>(from + (size_t)c * 2 * hidden, true));
+      W* row = grad_table + (size_t)key * hidden + (size_t)step * VEC;
+      if constexpr (ADD) store_stream_32<W, VEC>(row, sum.times_plus(scale, load_stream_32<W, VEC>(row, s.wide)), s.wide);
+      else store_stream_32<W, VEC>(row, sum.template times<W>(scale), s.wide);
+    }
+  }
   for (unsigned long long item = blockIdx.x; item < items; item += join_blocks) {
-    const size_t chunk = s.crossings[1 + item / tiles];
+    const size_t chunk = s.crossings[1 + s.chunks - item / tiles];
     const int step = (int)(item % tiles) * 32 + lane;
     const size_t column = (size_t)step * VEC;
     const uint32_t key = s.keys[(chunk + 1) * s.chunk_length - 1];
@@ -631,7 +659,7 @@ template <typename G, typename W, int VEC, bool ADD> int gradient(const Gradient
     s.chunk_length *= 2;
   s.chunks = (uint32_t)((count + s.chunk_length - 1) / s.chunk_length);
   const bool spare = count > 65536;
-  const size_t list = round_up(count * 4), crossings = round_up((1 + (size_t)s.chunks) * 4);
+  const size_t list = round_up(count * 4), crossings = round_up((2 + (size_t)s.chunks) * 4);
   const size_t counts_bytes = spare ? round_up((count + kTile - 1) / kTile * kBins * 4) : 0, partial = round_up((size_t)s.chunks * 2 * call.hidden * 4);
   const size_t named_bytes = ADD ? 0 : round_up(call.vocabulary);
   Workspace workspace(stream);
