@@ -49,8 +49,9 @@ def _lowered_module_type():
 
 
 def _bind_device(device_id: int) -> None:
-    """Make ``device_id``'s primary context current on this thread (once per thread/device)."""
-    if getattr(_thread_state, "device", None) != device_id:
+    """Make ``device_id``'s primary context current on this thread.  Where there is one device, once per thread; where there
+    are several, every time: the program may have made another one current in between."""
+    if getattr(_thread_state, "device", None) != device_id or native.several_devices():
         native.call("bb200_init", device_id)
         _thread_state.device = device_id
 
@@ -215,7 +216,8 @@ class B200Backend:
                         # that returned non-zero (upstream hipcc_exec.py:181-182)
                         status = native.take_device_status(stream_handle)
                         if status == native.TOKEN_OUT_OF_RANGE:
-                            raise RuntimeError(f"launch_{ir.name} returned device status {status}: a token lies outside the table's rows")
+                            raise RuntimeError(f"launch_{ir.name} returned device status {status}: a token of this lookup, or of one before "
+                                               "that was not waited for, lies outside the table")
                         if status:
                             raise RuntimeError(f"launch_{ir.name} returned device status {status}: a bounded device-side wait "
                                                f"gave up ({native.ERROR_NAMES[-6]}); the output is incomplete")

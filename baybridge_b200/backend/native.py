@@ -260,11 +260,17 @@ def device_available() -> bool:
 
 
 _device_seen = False
+_device_count = 0
+
+
+def several_devices() -> bool:
+    """Whether more than one CUDA device is visible (known once ``require_device`` has run)."""
+    return _device_count > 1
 
 
 def require_device() -> None:
     """Fail loudly (no fallback) when launches are impossible on this machine."""
-    global _device_seen
+    global _device_seen, _device_count
     if _device_seen:
         return
     count = ctypes.c_int(0)
@@ -273,4 +279,4 @@ def require_device() -> None:
     if status != 0 or count.value < 1:
         detail = (lib.bb200_last_error() or b"").decode("utf-8", "replace") if status else "no CUDA device is visible"
         raise BackendNotImplementedError(f"the b200 backend needs a CUDA device and driver: {detail}")
-    _device_seen = True
+    _device_seen, _device_count = True, count.value

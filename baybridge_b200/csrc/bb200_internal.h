@@ -119,6 +119,37 @@ class Workspace {
   char* data_ = nullptr;
 };
 
+// Whether the current device can hold a cluster of 16 CTAs of KERNEL (with `threads` threads and `shared_bytes` of dynamic
+// shared memory, the same in every call): beyond the portable eight, it depends on the multiprocessors that are there.
+// Asked once per kernel and device.
+template <auto KERNEL> bool sixteen_fit(int threads, size_t shared_bytes) {
+  static std::atomic<int> answers[kMaxWorkspaceDevices];  // 0: not asked yet, 1: no, 2: yes
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kMaxWorkspaceDevices) return false;
+  int answer = answers[device].load(std::memory_order_relaxed);
+  if (!answer) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(16);
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = shared_bytes;
+    cudaLaunchAttribute attribute = {};
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = 16;
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    int clusters = 0;
+    answer = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                     cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared_bytes) == cudaSuccess &&
+                     cudaOccupancyMaxActiveClusters(&clusters, KERNEL, &config) == cudaSuccess && clusters > 0
+                 ? 2
+                 : 1;
+    cudaGetLastError();  // a "no" is no error of the call
+    answers[device].store(answer, std::memory_order_relaxed);
+  }
+  return answer == 2;
+}
+
 // Raise KERNEL's limit of dynamic shared memory to `bytes` on the current device, once per kernel and device (`bytes` is the
 // same in every call; two threads doing it at once is harmless).
 template <auto KERNEL> int allow_shared_memory(int bytes, const char* what) {

@@ -584,11 +584,6 @@ template <typename Id, int R>
 int launch_cluster_sort(const GradientCall& call, unsigned ctas, int passes, int digit_bits, const SortedList& list, uint8_t* named, size_t zero_bytes,
                         cudaStream_t stream) {
   const unsigned fill = zero_bytes ? ((unsigned)multiprocessor_count() + ctas - 1) / ctas * ctas : 0;  // whole clusters
-  if (ctas > 8) {  // beyond the portable size; the attribute is cheap to set again
-    if (int status = check_runtime(cudaFuncSetAttribute(sort_in_cluster<Id, R>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
-                                   "cudaFuncSetAttribute(embedding_backward sort)"))
-      return status;
-  }
   if (int status = allow_shared_memory<sort_in_cluster<Id, R>>((int)sizeof(ClusterSort<R>), "cudaFuncSetAttribute(embedding_backward sort)")) return status;
   launch_dependent_cluster(sort_in_cluster<Id, R>, dim3(ctas + fill), dim3(kSortThreads), ctas, sizeof(ClusterSort<R>), stream,
                            static_cast<const Id*>(call.tokens), (uint32_t)call.count, (uint32_t)call.vocabulary, call.padding, passes, digit_bits,
@@ -605,15 +600,20 @@ int sort_tokens(const GradientCall& call, const SortedList& list, const SortedLi
   int bits = 1;  // of the keys 0 .. vocabulary
   while (((unsigned long long)call.vocabulary >> bits) != 0) ++bits;
   const int passes = (bits + kDigitBits - 1) / kDigitBits, digit_bits = (bits + passes - 1) / passes;
+  // Few elements a thread and many CTAs (65536 tokens: 24 us with 16 CTAs, 35 us with eight of twice the elements).
   const auto ctas = [count](uint32_t each) {  // a power of two
     unsigned n = 1;
     while (n * each < count) n *= 2;
     return n;
   };
-  // Few elements a thread and many CTAs: 65536 tokens 24 us with 16 CTAs, 35 us with eight of twice the elements.
-  if (count <= 16384) return launch_cluster_sort<Id, 1>(call, ctas(1024), passes, digit_bits, list, named, zero_bytes, stream);
-  if (count <= 32768) return launch_cluster_sort<Id, 2>(call, ctas(2048), passes, digit_bits, list, named, zero_bytes, stream);
-  if (count <= 65536) return launch_cluster_sort<Id, 4>(call, ctas(4096), passes, digit_bits, list, named, zero_bytes, stream);
+  const unsigned one = ctas(1024), two = ctas(2048), four = ctas(4096), eight = ctas(8192);
+  if (one <= 8 || (one == 16 && sixteen_fit<sort_in_cluster<Id, 1>>(kSortThreads, sizeof(ClusterSort<1>))))
+    return launch_cluster_sort<Id, 1>(call, one, passes, digit_bits, list, named, zero_bytes, stream);
+  if (two <= 8 || (two == 16 && sixteen_fit<sort_in_cluster<Id, 2>>(kSortThreads, sizeof(ClusterSort<2>))))
+    return launch_cluster_sort<Id, 2>(call, two, passes, digit_bits, list, named, zero_bytes, stream);
+  if (four <= 8 || (four == 16 && sixteen_fit<sort_in_cluster<Id, 4>>(kSortThreads, sizeof(ClusterSort<4>))))
+    return launch_cluster_sort<Id, 4>(call, four, passes, digit_bits, list, named, zero_bytes, stream);
+  if (eight <= 8) return launch_cluster_sort<Id, 8>(call, eight, passes, digit_bits, list, named, zero_bytes, stream);
   const Id* tokens = static_cast<const Id*>(call.tokens);
   const int tiles = (int)((call.count + kTile - 1) / kTile);
   const uint32_t mask = (1u << digit_bits) - 1;

@@ -275,10 +275,6 @@ template <typename T, typename Rows, bool RESIDUAL> int launch_cluster(const Bac
   if (int status = allow_shared_memory<kernel>(Rows::kBytes, "cudaFuncSetAttribute(layernorm_backward)")) return status;
   unsigned ctas = 1;
   while (ctas < kMostCtas && ctas < wanted) ctas *= 2;
-  if (ctas > 8) {  // beyond the portable size; the attribute is cheap to set again
-    if (int status = check_runtime(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "cudaFuncSetAttribute(layernorm_backward)"))
-      return status;
-  }
   launch_dependent_cluster(kernel, dim3(ctas), dim3(kRowThreads), ctas, (size_t)Rows::kBytes, stream, p);
   return check_launch("layernorm_backward kernel launch");
 }
@@ -286,7 +282,8 @@ template <typename T, typename Rows, bool RESIDUAL> int launch_cluster(const Bac
 template <typename T, typename Rows, bool RESIDUAL, bool MAY_CLUSTER> int launch_rows(Backward<T> p, cudaStream_t stream) {
   const size_t wanted = (p.rows + Rows::GROUPS - 1) / Rows::GROUPS, most = (size_t)multiprocessor_count();
   if constexpr (MAY_CLUSTER) {
-    if (wanted <= 2 * kMostCtas) return launch_cluster<T, Rows, RESIDUAL>(p, wanted, stream);
+    if (wanted <= 8 || (wanted <= 2 * kMostCtas && sixteen_fit<norm_backward_rows<T, Rows, RESIDUAL, true>>(kRowThreads, Rows::kBytes)))
+      return launch_cluster<T, Rows, RESIDUAL>(p, wanted, stream);
   }
   constexpr auto kernel = norm_backward_rows<T, Rows, RESIDUAL, false>;
   if (int status = allow_shared_memory<kernel>(Rows::kBytes, "cudaFuncSetAttribute(layernorm_backward)")) return status;

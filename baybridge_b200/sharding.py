@@ -40,8 +40,8 @@ class ShardSpec:
 
 def shard_spec(plan: Any, ir: Any) -> ShardSpec:
     """Sharding of a matched plan (see ``backend.matcher``): elementwise → flat chunks of axis 0, RMSNorm →
-    rows, GEMM → M (A and C by rows, B replicated), attention → batch, LayerNorm → rows, reductions that keep
-    the leading axis → rows (others do not shard)."""
+    rows, GEMM → M (A and C by rows, B replicated), attention → batch, LayerNorm → rows, embedding → the tokens' leading
+    axis (the table replicated), reductions that keep the leading axis → rows (others do not shard)."""
     kind = plan.kind
     if kind == "elementwise":
         if plan.mode != "flat":
@@ -86,6 +86,21 @@ def shard_spec(plan: Any, ir: Any) -> ShardSpec:
         shared = tuple(p for p, is_full in ((plan.weight, plan.weight_is_full), (plan.bias, plan.bias_is_full)) if not is_full)
         return ShardSpec(kind, shape[0], tuple((p, 0) for p in per_row + full), shared, (plan.out, plan.out_resid),
                          reads=(plan.x, plan.residual, plan.weight, plan.bias))
+    if kind == "embedding":
+        tokens = ir.arguments[plan.tokens].spec.shape
+        if not tokens:
+            raise ValueError("the lookup of a single token does not shard")
+        return ShardSpec(kind, tokens[0], ((plan.tokens, 0), (plan.out, 0)), (plan.table,), (plan.out,), reads=(plan.tokens, plan.table))
+    if kind == "layernorm_forward":
+        shape = ir.arguments[plan.x].spec.shape
+        if len(shape) < 2:
+            raise ValueError("a rank-1 layernorm has a single row and does not shard")
+        given = lambda *positions: tuple(p for p in positions if p is not None)  # noqa: E731
+        outputs = given(plan.out, plan.out_resid, plan.mean, plan.rstd)
+        return ShardSpec(kind, shape[0], tuple((p, 0) for p in given(plan.x, plan.residual) + outputs), given(plan.weight, plan.bias), outputs,
+                         reads=given(plan.x, plan.residual, plan.weight, plan.bias))
+    if kind in ("embedding_backward", "layernorm_backward", "adamw"):
+        raise ValueError(f"{kind} sums or steps over the whole batch or all parameters; it does not shard without an exchange step")
     if kind == "reduction_bundle":
         raise ValueError("a bundle of reductions folds over different axes of one tensor; it does not shard")
     if kind == "reduction":

@@ -128,6 +128,33 @@ def test_unaligned_tensors_and_their_neighbours():
         assert bool((flat[mask] == 7).all())
 
 
+@pytest.mark.parametrize("offset", [4, 8])
+def test_tensors_aligned_to_16_bytes_but_not_to_32(offset):
+    torch = _torch()
+    for param, grad, masters in (("f32", "f32", False), ("bf16", "f32", True)):
+        lists = Lists([((5000,), param, grad), ((4097,), param, grad)], masters, seed=8)
+        for name in ("params", "grads", "exp_avgs", "exp_avg_sqs", "masters"):
+            values = getattr(lists, name)
+            if values is None:
+                continue
+            views = []
+            for value in values:
+                start = offset if value.dtype == torch.float32 else 2 * offset
+                views.append(torch.zeros(value.numel() + 64, device="cuda", dtype=value.dtype)[start:start + value.numel()])
+                views[-1].copy_(value)
+            setattr(lists, name, views)
+        check = lists.expect()
+        lists.compile()(*lists.arguments())
+        check()
+
+
+def test_a_parameter_without_an_axis():
+    lists = Lists([((), "f32", "f32"), ((2,), "f32", "f32")], seed=9)
+    check = lists.expect()
+    lists.compile()(*lists.arguments())
+    check()
+
+
 @pytest.mark.parametrize("betas,epsilon,step", [((0.0, 0.0), 1e-6, 1.0), ((0.9, 0.999), 1e-8, 1.0), ((0.95, 0.99), 1e-8, 100000.0), ((0.5, 0.9999), 0.1, 7.0)])
 def test_schedule_and_constants(betas, epsilon, step):
     lists = Lists([((500,), "f32", "f32")], seed=4, decay=0.0)

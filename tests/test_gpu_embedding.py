@@ -151,7 +151,8 @@ GRADIENT_SHAPES = [
     # count, vocabulary, hidden, kind
     (1, 1, 1, "even"), (1, 1000, 8, "even"), (3, 2, 7, "even"), (31, 5, 64, "zipf"), (32, 40, 129, "zipf"), (33, 1, 520, "same"),
     (257, 300, 8, "zipf"), (1000, 2000, 96, "distinct"), (4096, 512, 64, "zipf"), (4097, 513, 40, "zipf"), (5000, 131072, 16, "even"),
-    (8192, 100, 33, "same"), (20000, 50257, 24, "zipf"), (70000, 1 << 20, 8, "zipf"), (70000, 3, 17, "even"), (600000, 1000, 8, "zipf"),
+    (8192, 100, 33, "same"), (16384, 700, 12, "zipf"), (20000, 50257, 24, "zipf"), (32769, 131072, 16, "zipf"), (65536, 999, 8, "even"),
+    (65537, 999, 8, "zipf"), (3000, 40, 1032, "zipf"), (50000, 17, 264, "zipf"), (70000, 1 << 20, 8, "zipf"), (70000, 3, 17, "even"), (600000, 1000, 8, "zipf"),
 ]
 
 
@@ -217,6 +218,72 @@ def test_infinite_and_nan_gradients_stay_in_their_rows():
     assert bool(table[1, 5].isinf()) and bool(table[2, 6].isnan())
     table[1, 5] = table[2, 6] = 0
     assert bool(table.isfinite().all())
+
+
+@pytest.mark.parametrize("offset", [4, 8])
+@pytest.mark.parametrize("grad_dtype,table_dtype", [("f32", "f32"), ("bf16", "f32"), ("f32", "bf16")])
+def test_tensors_aligned_to_16_bytes_but_not_to_32(offset, grad_dtype, table_dtype):
+    torch = _torch()
+    count, vocabulary, hidden = 700, 60, 48
+    tokens = _tokens(count, vocabulary, "i32", 90)
+
+    def shifted(shape, dtype, seed):
+        flat = torch.full((shape[0] * shape[1] + 32,), 9.0, device="cuda", dtype=_dtype(dtype))
+        start = offset if dtype == "f32" else 2 * offset
+        view = flat[start:start + shape[0] * shape[1]].view(shape)
+        view.copy_(_rows(shape, dtype, seed))
+        return flat, start, view
+
+    _, _, grad = shifted((count, hidden), grad_dtype, 91)
+    flat, start, table = shifted((vocabulary, hidden), table_dtype, 92)
+    for accumulate in (True, False):
+        expected, error, _ = _expected_gradient(grad, tokens, table, 1.0, None, accumulate)
+        _gradient(grad, tokens, table, accumulate=accumulate)(grad, tokens, table)
+        within(table, expected, table_dtype, error)
+    out_flat, out_start, out = shifted((count, hidden), grad_dtype, 93)
+    _lookup(tokens, table, out)(tokens, table, out)
+    within(out, table.double()[tokens.long()], grad_dtype, 0 * table.double()[tokens.long()])
+    for storage, first, view in ((flat, start, table), (out_flat, out_start, out)):
+        assert bool((storage[:first] == 9).all()) and bool((storage[first + view.numel():] == 9).all())
+
+
+def test_a_single_token_without_an_axis():
+    torch = _torch()
+    table, token = _rows((30, 40), "f32", 95), torch.tensor(7, device="cuda")
+    out, grad_table = torch.empty(40, device="cuda"), torch.empty(30, 40, device="cuda")
+    _lookup(token, table, out, scale=2.0)(token, table, out)
+    assert torch.equal(out, table[7] * 2)
+    _gradient(out, token, grad_table)(out, token, grad_table)
+    assert torch.equal(grad_table[7], out) and not grad_table[:7].any() and not grad_table[8:].any()
+
+
+def test_gradient_inside_a_torch_graph():
+    """Captured by another program's graph: the workspace becomes the graph's own."""
+    torch = _torch()
+    import baybridge_b200 as cute
+
+    tokens, grad, table = _tokens(3000, 400, "i32", 96), _rows((3000, 24), "f32", 97), torch.zeros(400, 24, device="cuda")
+
+    @cute.kernel
+    def gradient(grad_out: cute.Tensor, tokens: cute.Tensor, grad_table: cute.Tensor):
+        cute.embedding_backward(grad_out, tokens, grad_table)
+
+    handles = [cute.from_dlpack(t) for t in (grad, tokens, table)]
+    artifact = cute.compile(gradient, *handles, backend=cute.B200Backend(synchronize=False))
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        artifact(*handles, stream=side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        artifact(*handles, stream=side)
+    for seed in (98, 99):
+        grad.copy_(_rows((3000, 24), "f32", seed))
+        graph.replay()
+        graph.replay()
+        torch.cuda.synchronize()
+        expected, error, _ = _expected_gradient(grad, tokens, table, 1.0, None, False)
+        within(table, expected, "f32", error)
 
 
 def test_calls_on_two_streams_do_not_share_a_workspace():

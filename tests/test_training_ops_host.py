@@ -4,6 +4,7 @@ from __future__ import annotations
 import ctypes
 
 import pytest
+from test_fake_driver import ELEMENTWISE_CHILD, calls, fake_driver, run_child  # noqa: F401 - a fixture among them
 from test_host_surface import FakeCudaTensor
 
 import baybridge_b200 as cute
@@ -173,3 +174,98 @@ def test_c_abi_checks_its_arguments_before_any_device_work():
     assert adamw(count=0) == -1 and adamw(numel=0) == -1 and adamw(kinds=(3, 3)) == -1 and adamw(kinds=(0, 1)) == -1 and adamw(beta1=1.0) == -1
     assert adamw(epsilon=float("nan")) == -1 and adamw(addresses=(K, 2 * K, 3 * K, 4 * K, 0)) == -1 and adamw(addresses=(K + 1, 2 * K, 3 * K, 4 * K, 5 * K)) == -3
     assert adamw(addresses=(K, K, 3 * K, 4 * K, 5 * K)) == -1 and adamw(addresses=(K, 2 * K, 3 * K, 3 * K + 128, 5 * K)) == -1
+
+
+def test_lookups_and_norms_shard_by_rows_and_what_sums_over_them_does_not(tmp_path, zoo):
+    from baybridge_b200.sharding import shard_spec
+
+    x, stat, w = tensor((6, 4, 16), "bfloat16"), tensor((6, 4)), tensor((16,))
+    tokens, table = tensor((6, 4), "int32"), tensor((9, 16), "bfloat16")
+
+    def spec_of(kernel, *arguments):
+        ir = cute.compile(kernel, *arguments, backend="portable", cache_dir=tmp_path).ir
+        return shard_spec(match(ir), ir)
+
+    lookup = spec_of(zoo.make_embedding(), tokens, table, x)
+    assert (lookup.extent, lookup.sharded, lookup.replicated, lookup.outputs, lookup.reads) == (6, ((0, 0), (2, 0)), (1,), (2,), (0, 1))
+    norm = spec_of(zoo.layernorm_forward, x, x, stat, stat, w, w)
+    assert (norm.extent, norm.sharded, norm.replicated, norm.outputs) == (6, ((0, 0), (1, 0), (2, 0), (3, 0)), (4, 5), (1, 2, 3))
+    for kernel, arguments in ((zoo.make_embedding_backward(), (x, tokens, table)), (zoo.layernorm_backward, (x, x, stat, stat, w, x, w, w)),
+                              (zoo.make_adamw(), ([w], [w], [w], [w], tensor((3,))))):
+        with pytest.raises(ValueError, match="does not shard"):
+            spec_of(kernel, *arguments)
+
+
+def test_a_launch_binds_its_tensors_device_again_where_another_was_made_current(fake_driver, tmp_path):  # noqa: F811
+    """Two devices: between two launches on device 0 the program makes device 1 current; the second launch has to make
+    device 0 current again.  With one device nothing is bound twice."""
+    body = ELEMENTWISE_CHILD + """
+    tensors = [FakeCudaTensor((n,), "float32", 0x10000 * (i + 1), 0) for i in range(3)]
+    artifact = cute.compile(zoo.make_indexed_binary("add", n), *tensors, backend="b200", cache_dir=%r)
+    artifact(*tensors)
+    if %d > 1:
+        native.call("bb200_init", 1)
+    artifact(*tensors)
+    result = {}
+    """
+    _, log = run_child(fake_driver, tmp_path, body % (str(tmp_path / "cache"), 2), devices=2)
+    launches = [i for i, line in enumerate(log) if line.startswith("cuLaunchKernelEx")]
+    for launch in launches:
+        assert [line for line in log[:launch] if line.startswith("cuCtxSetCurrent")][-1] == "cuCtxSetCurrent context=0xc0de0000"
+    (tmp_path / "driver_calls.log").unlink()
+    _, log = run_child(fake_driver, tmp_path, body % (str(tmp_path / "cache"), 1), devices=1)
+    assert len(calls(log, "cuCtxSetCurrent")) == 1
+
+
+def test_launchers_take_the_short_path_only_for_what_they_were_compiled_for(tmp_path, zoo, monkeypatch):
+    """Handles of the expected shapes go straight to the entry point; a wrong shape, dtype, device or number of arguments
+    raises as on the long path."""
+    seen = []
+
+    class Entry:
+        def __call__(self, *arguments):
+            seen.append(arguments)
+            return 0
+
+    monkeypatch.setattr(native, "entry_point", lambda name: Entry())
+    monkeypatch.setattr(native, "require_device", lambda: None)
+    monkeypatch.setattr("baybridge_b200.backend.b200._bind_device", lambda device: None)
+    tokens, table, out = (cute.from_dlpack(t) for t in (tensor((4,), "int32", 1 << 20), tensor((9, 16), ptr=2 << 20), tensor((4, 16), ptr=3 << 20)))
+    artifact = cute.compile(zoo.make_embedding(2.0), tokens, table, out, backend=cute.B200Backend(synchronize=False), cache_dir=tmp_path)
+    artifact(tokens, table, out)
+    artifact(tokens, table, out, stream=77)
+    artifact(tensor((4,), "int32", 1 << 20), tensor((9, 16), ptr=2 << 20), tensor((4, 16), ptr=3 << 20))  # exporters, not handles
+    assert [a[3:6] for a in seen] == [(1 << 20, 2 << 20, 3 << 20)] * 3 and seen[0][-1] is None and seen[1][-1].value == 77
+    with pytest.raises(TypeError, match="expects f32"):
+        artifact(tokens, cute.from_dlpack(tensor((9, 17), ptr=2 << 20)), out)
+    with pytest.raises(TypeError, match="expects f32"):
+        artifact(tokens, cute.from_dlpack(tensor((9, 16), "bfloat16", 2 << 20)), out)
+    with pytest.raises(cute.BackendNotImplementedError, match="different devices"):
+        artifact(tokens, cute.from_dlpack(tensor((9, 16), ptr=2 << 20, device=(2, 1))), out)
+    with pytest.raises(cute.BackendNotImplementedError, match="contiguous"):
+        artifact(tokens, cute.from_dlpack(tensor((9, 16), ptr=2 << 20, stride=(1, 9))), out)
+    with pytest.raises((TypeError, KeyError)):
+        artifact(tokens, table)
+    assert len(seen) == 3
+
+
+def test_groups_of_adamw_reach_the_entry_point_whole_and_are_compared(tmp_path, zoo, monkeypatch):
+    seen = []
+    monkeypatch.setattr(native, "entry_point", lambda name: lambda *arguments: seen.append(arguments) or 0)
+    monkeypatch.setattr(native, "require_device", lambda: None)
+    monkeypatch.setattr("baybridge_b200.backend.b200._bind_device", lambda device: None)
+    place = iter(range(1 << 20, 1 << 30, 1 << 16))
+    lists = [cute.tensor_group([tensor(s, ptr=next(place)) for s in ((3, 5), (7,))]) for _ in range(4)]
+    schedule = cute.from_dlpack(tensor((3,), ptr=next(place)))
+    artifact = cute.compile(zoo.make_adamw(), *lists, schedule, backend=cute.B200Backend(synchronize=False), cache_dir=tmp_path)
+    artifact(*lists, schedule)
+    artifact(*[list(group) for group in lists], schedule)
+    for arguments in seen:
+        assert arguments[0] == 2 and [list(array) for array in arguments[5:9]] == [list(group.addresses) for group in lists] and arguments[9] is None
+    short = cute.tensor_group([lists[0][0]])
+    with pytest.raises(TypeError, match="the params of adamw_kernel differ"):
+        artifact(short, *lists[1:], schedule)
+    other = cute.tensor_group([tensor(s, ptr=next(place), device=(2, 1)) for s in ((3, 5), (7,))])
+    with pytest.raises(cute.BackendNotImplementedError, match="different devices"):
+        artifact(other, *lists[1:], schedule)
+    assert len(seen) == 2
