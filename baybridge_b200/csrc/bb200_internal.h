@@ -19,36 +19,44 @@ int check_runtime(cudaError_t err, const char* what);
 // After a kernel launch: pick up launch-configuration errors without synchronising.
 inline int check_launch(const char* what) { return check_runtime(cudaGetLastError(), what); }
 
-// Launch `kernel` with programmatic stream serialisation: its CTAs may be placed while the kernel before it on `stream`
-// drains.  ONLY for kernels that run `dependent_launch_prologue()` (below) before their first global-memory access.
-// A capturing stream takes the ordinary launch.  `cluster`: CTAs of a cluster along x.
+// The configuration of a launch with programmatic stream serialisation: the kernel's CTAs may be placed while the kernel
+// before it on `stream` drains.  ONLY for kernels that run `dependent_launch_prologue()` (below) before their first
+// global-memory access.  A capturing stream takes the ordinary launch.  `cluster`: CTAs of a cluster along x.
+struct DependentLaunch {
+  cudaLaunchConfig_t config = {};
+  cudaLaunchAttribute attributes[2] = {};
+  DependentLaunch(dim3 grid, dim3 block, unsigned cluster, size_t dynamic_smem, cudaStream_t stream) {
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    const bool capturing = cudaStreamIsCapturing(stream, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone;
+    config.gridDim = grid;
+    config.blockDim = block;
+    config.dynamicSmemBytes = dynamic_smem;
+    config.stream = stream;
+    config.attrs = attributes;
+    if (!capturing) {
+      attributes[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attributes[config.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+      attributes[config.numAttrs].id = cudaLaunchAttributeClusterDimension;
+      attributes[config.numAttrs].val.clusterDim.x = cluster;
+      attributes[config.numAttrs].val.clusterDim.y = 1;
+      attributes[config.numAttrs++].val.clusterDim.z = 1;
+    }
+  }
+  DependentLaunch(const DependentLaunch&) = delete;  // config points to attributes
+  DependentLaunch& operator=(const DependentLaunch&) = delete;
+};
+
 template <typename... Params, typename... Args>
 inline void launch_dependent_cluster(void (*kernel)(Params...), dim3 grid, dim3 block, unsigned cluster, size_t dynamic_smem,
-                                     cudaStream_t stream, Args... args) {
-  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-  const bool capturing = cudaStreamIsCapturing(stream, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = grid;
-  config.blockDim = block;
-  config.dynamicSmemBytes = dynamic_smem;
-  config.stream = stream;
-  cudaLaunchAttribute attributes[2] = {};
-  config.attrs = attributes;
-  if (!capturing) {
-    attributes[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attributes[config.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
-  }
-  if (cluster > 1) {
-    attributes[config.numAttrs].id = cudaLaunchAttributeClusterDimension;
-    attributes[config.numAttrs].val.clusterDim.x = cluster;
-    attributes[config.numAttrs].val.clusterDim.y = 1;
-    attributes[config.numAttrs++].val.clusterDim.z = 1;
-  }
-  cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);  // the caller reads the status with check_launch()
+                                     cudaStream_t stream, const Args&... args) {
+  DependentLaunch launch(grid, block, cluster, dynamic_smem, stream);
+  cudaLaunchKernelEx(&launch.config, kernel, static_cast<Params>(args)...);  // the caller reads the status with check_launch()
 }
 
 template <typename... Params, typename... Args>
-inline void launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, size_t dynamic_smem, cudaStream_t stream, Args... args) {
+inline void launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, size_t dynamic_smem, cudaStream_t stream, const Args&... args) {
   launch_dependent_cluster(kernel, grid, block, 1, dynamic_smem, stream, args...);
 }
 
