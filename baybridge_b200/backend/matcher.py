@@ -503,7 +503,7 @@ def _norm_shapes(x_spec, same, vectors, stats, what: str) -> tuple[int, int]:
         raise _unsupported(f"{what} requires its row tensors of one shape and dtype")
     if any(spec.shape != (hidden,) or spec.dtype != vectors[0].dtype or spec.dtype not in (x_spec.dtype, "f32") for spec in vectors):
         raise _unsupported(f"{what} requires weight and bias vectors [hidden] of one dtype, x's or f32")
-    if any(spec.numel != rows or spec.dtype != "f32" for spec in stats):
+    if any(spec.shape != (x_spec.shape[:-1] or (1,)) or spec.dtype != "f32" for spec in stats):
         raise _unsupported(f"{what} requires f32 mean and rstd, one value per row")
     limit = 16384 if x_spec.dtype == "f32" else 32768
     if hidden > limit or rows >= 2**31 - 1:

@@ -9,6 +9,9 @@
 // finds its tensor by a binary search over the tensors' first tiles.  rate, step and factor are read from device
 // memory.  All arithmetic is fp32; 1 - beta^step is -expm1(step log beta), which keeps its digits for beta near 1.
 #include <math.h>
+#include <stdlib.h>
+
+#include <algorithm>
 
 #include "bb200_internal.h"
 #include "bb200_rows.cuh"
@@ -204,6 +207,49 @@ template <typename P, typename G> int launch_kind(const Call& call, int param_co
                                  : launch_pair<P, G, false, kLargeTable>(call, param_code, grad_code, stream);
 }
 
+struct Span {
+  uintptr_t begin, end;
+};
+
+// Refuses tensors that share memory, whichever lists they come from: two CTAs would step the same elements.  The lists are
+// sorted by address one by one (mostly they are already: allocated one after the other) and merged where they interleave,
+// so a call costs a few passes over them.
+int check_disjoint(const Call& call) {
+  const void* const* const lists[] = {call.params, call.grads, const_cast<const void* const*>(call.exp_avgs),
+                                      const_cast<const void* const*>(call.exp_avg_sqs), const_cast<const void* const*>(call.masters)};
+  const size_t used = call.masters ? 5 : 4, count = (size_t)call.count, all = used * count + 1;
+  Span* const buffer = static_cast<Span*>(malloc(2 * all * sizeof(Span)));
+  if (!buffer) return fail(BB200_E_INVALID_ARGUMENT, "adamw: no host memory for a table of %zu tensors", all);
+  Span *spans = buffer, *other = buffer + all;
+  const auto before = [](const Span& a, const Span& b) { return a.begin < b.begin; };
+  const auto append = [&](size_t have, size_t more) {
+    Span* added = spans + have;
+    if (!std::is_sorted(added, added + more, before)) std::sort(added, added + more, before);
+    if (have && added[0].begin < added[-1].begin) {
+      std::merge(spans, added, added, added + more, other, before);
+      std::swap(spans, other);
+    }
+  };
+  for (size_t list = 0; list < used; ++list) {
+    const int* dtypes = list == 0 ? call.param_dtypes : list == 1 ? call.grad_dtypes : nullptr;
+    Span* added = spans + list * count;
+    for (size_t i = 0; i < count; ++i) {
+      const uintptr_t begin = reinterpret_cast<uintptr_t>(lists[list][i]);
+      added[i] = {begin, begin + (dtypes && dtypes[i] != BB200_F32 ? 2 : 4) * call.numels[i]};
+    }
+    append(list * count, count);
+  }
+  const uintptr_t schedule = reinterpret_cast<uintptr_t>(call.schedule);
+  spans[all - 1] = {schedule, schedule + 3 * sizeof(float)};
+  append(all - 1, 1);
+  size_t k = 1;
+  while (k < all && spans[k - 1].end <= spans[k].begin) ++k;
+  const uintptr_t first = spans[k - 1].begin, second = k < all ? spans[k].begin : 0;
+  free(buffer);
+  if (k == all) return BB200_OK;
+  return fail(BB200_E_INVALID_ARGUMENT, "adamw: two of the tensors (the schedule among them) share memory: at %#zx and %#zx", (size_t)first, (size_t)second);
+}
+
 }  // namespace
 }  // namespace bb200
 
@@ -223,21 +269,18 @@ extern "C" int bb200_adamw(int count, const size_t* numels, const int* param_dty
       return fail(BB200_E_INVALID_ARGUMENT, "adamw: tensor %d has dtypes %d and %d; parameters are bf16/f16/f32, gradients alike or f32", i, p, g);
     if (numels[i] == 0) return fail(BB200_E_INVALID_ARGUMENT, "adamw: tensor %d is empty", i);
     if (numels[i] > (size_t)kTileElements * 0x7fffffffu) return fail(BB200_E_UNSUPPORTED_SHAPE, "adamw: tensor %d is too large", i);
-    const size_t param_bytes = numels[i] * dtype_bytes((bb200_dtype)p), grad_bytes = numels[i] * dtype_bytes((bb200_dtype)g), wide = numels[i] * 4;
-    const struct { const void* p; size_t bytes, size; } tensors[5] = {
-        {params[i], param_bytes, dtype_bytes((bb200_dtype)p)}, {exp_avgs[i], wide, 4}, {exp_avg_sqs[i], wide, 4},
-        {masters ? masters[i] : nullptr, wide, 4}, {grads[i], grad_bytes, dtype_bytes((bb200_dtype)g)}};
-    for (int a = 0; a < 5; ++a) {
-      if (!tensors[a].p && !(a == 3 && !masters)) return fail(BB200_E_INVALID_ARGUMENT, "adamw: tensor %d has a null pointer", i);
+    const struct { const void* p; size_t size; } tensors[5] = {{params[i], dtype_bytes((bb200_dtype)p)}, {grads[i], dtype_bytes((bb200_dtype)g)},
+                                                               {exp_avgs[i], 4}, {exp_avg_sqs[i], 4}, {masters ? masters[i] : nullptr, 4}};
+    for (int a = 0; a < (masters ? 5 : 4); ++a) {
+      if (!tensors[a].p) return fail(BB200_E_INVALID_ARGUMENT, "adamw: tensor %d has a null pointer", i);
       if (reinterpret_cast<uintptr_t>(tensors[a].p) % tensors[a].size)
         return fail(BB200_E_MISALIGNED, "adamw: tensor %d is not aligned to its element size", i);
-      for (int b = 0; b < a; ++b)
-        if (overlap(tensors[a].p, tensors[a].bytes, tensors[b].p, tensors[b].bytes))
-          return fail(BB200_E_INVALID_ARGUMENT, "adamw: two of the tensors number %d share memory", i);
     }
   }
+  if (reinterpret_cast<uintptr_t>(schedule) % sizeof(float)) return fail(BB200_E_MISALIGNED, "adamw: the schedule is not aligned to its element size");
   const Call call = {count, numels, param_dtypes, grad_dtypes, weight_decays, params, grads, exp_avgs, exp_avg_sqs, masters, schedule,
                      beta1, beta2, epsilon};
+  if (int status = check_disjoint(call)) return status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (int status = launch_kind<float, float>(call, BB200_F32, BB200_F32, s)) return status;
   if (int status = launch_kind<__nv_bfloat16, __nv_bfloat16>(call, BB200_BF16, BB200_BF16, s)) return status;

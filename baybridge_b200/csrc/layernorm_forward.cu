@@ -372,8 +372,12 @@ template <typename T> int forward(const Forward<T>& p, bool aligned, cudaStream_
     BB200_VECTOR_ROWS(256, 4);
     if constexpr (VEC == 4) BB200_VECTOR_ROWS(512, 4);
 #undef BB200_VECTOR_ROWS
-    if (nvec <= 2048) launch_dependent(norm_long_rows<T, 1024, 2>, dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
-    else launch_dependent(norm_long_rows<T, 1024, 4>, dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
+    const dim3 grid((unsigned)p.rows), block(1024);
+    if (VEC == 8 && nvec <= 2048) {
+      if constexpr (VEC == 8) launch_dependent(norm_long_rows<T, 1024, 2>, grid, block, 0, stream, p);
+    } else {
+      launch_dependent(norm_long_rows<T, 1024, 4>, grid, block, 0, stream, p);
+    }
     return check_launch("layernorm_forward kernel launch");
   }
   // Other rows: a brief CTA for a few of them takes the fewest microseconds, the persistent form moves more bytes a second
@@ -398,8 +402,10 @@ template <typename T> int forward(const Forward<T>& p, bool aligned, cudaStream_
   if (p.hidden <= 2048) return launch_by_element<T, 256, 1, 8, 4>(p, stream);
   if (p.hidden <= 4096) return launch_by_element<T, 512, 1, 8, 4>(p, stream);
   if (p.hidden <= 8192) return launch_by_element<T, 1024, 1, 8, 4>(p, stream);
-  if (p.hidden <= 16384) return launch_by_element<T, 1024, 1, 16, 8>(p, stream);
-  return launch_by_element<T, 1024, 1, 32, 16>(p, stream);
+  if constexpr (VEC == 8) {  // rows of f32 end at 16384
+    if (p.hidden > 16384) return launch_by_element<T, 1024, 1, 32, 16>(p, stream);
+  }
+  return launch_by_element<T, 1024, 1, 16, 8>(p, stream);
 }
 
 }  // namespace

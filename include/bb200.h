@@ -353,8 +353,7 @@ int bb200_layernorm_backward(bb200_dtype dtype, bb200_dtype weight_dtype, const 
  * parameter is bf16 / f16 / f32 (param_dtypes[i]), its gradient alike or f32, its moments f32.  With `masters` (else NULL)
  * the step is taken on the f32 copies and the parameters receive them rounded.  schedule: device array {rate, step,
  * factor}, f32, step counted from 1; it is read when the kernel runs, so a recorded step replays with new values.  No two
- * of the tensors may share memory (checked among the tensors of one index).  One launch per 512 tensors of a pair of
- * dtypes.  No upstream counterpart. */
+ * of the tensors, the schedule among them, may share memory.  One launch per 512 tensors of a pair of dtypes.  No upstream counterpart. */
 int bb200_adamw(int count, const size_t* numels, const int* param_dtypes, const int* grad_dtypes, const float* weight_decays,
                 void* const* params, const void* const* grads, void* const* exp_avgs, void* const* exp_avg_sqs, void* const* masters,
                 const float* schedule, double beta1, double beta2, float epsilon, void* stream);

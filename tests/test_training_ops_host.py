@@ -176,6 +176,27 @@ def test_c_abi_checks_its_arguments_before_any_device_work():
     assert adamw(addresses=(K, K, 3 * K, 4 * K, 5 * K)) == -1 and adamw(addresses=(K, 2 * K, 3 * K, 3 * K + 128, 5 * K)) == -1
 
 
+@pytest.mark.parametrize("order", [(0, 1, 2), (2, 0, 1)])
+@pytest.mark.parametrize("which", [(0, 0, 0, 1), (0, 0, 1, 2), (1, 2, 3, 0), (2, 1, 4, 1), (4, 0, 4, 2), (0, 1, 5, 0)])
+def test_adamw_refuses_tensors_that_share_memory_across_indices_and_lists(which, order):
+    """Three tensors of 64 f32 in each of five lists, in rising or mixed order of address; one of them moved onto the last
+    element of another (list 5: the schedule)."""
+    K = 1 << 20
+    schedule = 64 * K
+    lists = [[K * (1 + 3 * role + place) for place in order] for role in range(5)]
+    from_list, from_index, to_list, to_index = which
+    lists[from_list][from_index] = schedule if to_list == 5 else lists[to_list][to_index] + 252
+    arrays = [(ctypes.c_void_p * 3)(*addresses) for addresses in lists]
+    f32 = (ctypes.c_int * 3)(0, 0, 0)
+    status = native.library().bb200_adamw(3, (ctypes.c_size_t * 3)(64, 64, 64), f32, f32, (ctypes.c_float * 3)(0, 0, 0), *arrays, _p(schedule),
+                                          0.9, 0.999, 1e-8, None)
+    assert status == -1 and b"share memory" in native.library().bb200_last_error()
+    aligned = [(ctypes.c_void_p * 3)(*[K * (1 + 3 * role + place) for place in order]) for role in range(5)]
+    status = native.library().bb200_adamw(3, (ctypes.c_size_t * 3)(64, 64, 64), f32, f32, (ctypes.c_float * 3)(0, 0, 0), *aligned, _p(schedule + 2),
+                                          0.9, 0.999, 1e-8, None)
+    assert status == -3
+
+
 def test_lookups_and_norms_shard_by_rows_and_what_sums_over_them_does_not(tmp_path, zoo):
     from baybridge_b200.sharding import shard_spec
 
