@@ -368,6 +368,12 @@ template <typename T> int forward(const Forward<T>& p, bool aligned, cudaStream_
     BB200_VECTOR_ROWS(32, 2);
     BB200_VECTOR_ROWS(32, 4);
     BB200_VECTOR_ROWS(64, 4);
+    // Around 4096 columns of 16 bits: four groups of 128 threads, which hide each other's sums (65536 x 4096 bf16: 177 us, with
+    // two of 256 259 us), but with a residual there is as much in flight either way, and the longer rows a group has in hand
+    // cost more than that (373 and 349 us); a few rows take the groups that finish one sooner (200 rows: 8.0 and 6.4 us).
+    if (!p.residual && p.rows > 2 * (size_t)multiprocessor_count()) {
+      if (nvec <= 512) return launch_rows<T, VectorRows<T, kRowThreads, 128, 4, 1, kMostSmem>, false>(p, stream);
+    }
     BB200_VECTOR_ROWS(256, 2);
     BB200_VECTOR_ROWS(256, 4);
     if constexpr (VEC == 4) BB200_VECTOR_ROWS(512, 4);

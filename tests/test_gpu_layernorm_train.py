@@ -57,7 +57,7 @@ SHAPES = [  # dtype, weight dtype, shape, residual, bias
     ("bf16", "f32", (13, 4096), True, True), ("f32", "f32", (9, 4096), False, True), ("bf16", "bf16", (700, 8192), True, True),
     ("f32", "f32", (5, 8192), True, False), ("f16", "f16", (3, 8200), False, True), ("bf16", "f32", (4, 16384), False, True),
     ("f32", "f32", (3, 16384), True, True), ("f16", "f32", (2, 32768), True, True), ("bf16", "bf16", (2, 32767), False, True),
-    ("f32", "f32", (2, 16383), True, True), ("bf16", "f32", (40000, 24), False, True),
+    ("f32", "f32", (2, 16383), True, True), ("bf16", "f32", (40000, 24), False, True), ("bf16", "f32", (701, 4000), False, True),
 ]
 
 
