@@ -153,6 +153,11 @@ GRADIENT_SHAPES = [
     (257, 300, 8, "zipf"), (1000, 2000, 96, "distinct"), (4096, 512, 64, "zipf"), (4097, 513, 40, "zipf"), (5000, 131072, 16, "even"),
     (8192, 100, 33, "same"), (16384, 700, 12, "zipf"), (20000, 50257, 24, "zipf"), (32769, 131072, 16, "zipf"), (65536, 999, 8, "even"),
     (65537, 999, 8, "zipf"), (3000, 40, 1032, "zipf"), (50000, 17, 264, "zipf"), (70000, 1 << 20, 8, "zipf"), (70000, 3, 17, "even"), (600000, 1000, 8, "zipf"),
+    # up to 1024 tokens: runs of one token on both sides of 16, rows of several column tiles, many rows that no token names
+    (1024, 3, 520, "even"), (1023, 1, 1032, "same"), (1024, 64, 264, "even"), (300, 3, 261, "even"), (1024, 1024, 136, "distinct"),
+    (16, 1, 40, "same"), (17, 1, 40, "same"), (1025, 7, 40, "even"), (9, 70001, 36, "even"), (1000, 300000, 3, "zipf"),
+    # as few tokens, of many columns: sorted all the same
+    (900, 50, 1061, "zipf"), (30, 4, 40000, "even"), (1, 3, 80000, "even"),
 ]
 
 
