@@ -222,26 +222,33 @@ int check_disjoint(const Call& call) {
   if (!buffer) return fail(BB200_E_INVALID_ARGUMENT, "adamw: no host memory for a table of %zu tensors", all);
   Span *spans = buffer, *other = buffer + all;
   const auto before = [](const Span& a, const Span& b) { return a.begin < b.begin; };
-  const auto append = [&](size_t have, size_t more) {
+  const auto append = [&](size_t have, size_t more, bool rising) {
     Span* added = spans + have;
-    if (!std::is_sorted(added, added + more, before)) std::sort(added, added + more, before);
+    if (!rising) std::sort(added, added + more, before);
     if (have && added[0].begin < added[-1].begin) {
       std::merge(spans, added, added, added + more, other, before);
       std::swap(spans, other);
     }
   };
-  for (size_t list = 0; list < used; ++list) {
+  size_t order[] = {0, 1, 2, 3, 4};  // by the first addresses: lists that lie apart need no merging then
+  std::sort(order, order + used, [&](size_t a, size_t b) { return reinterpret_cast<uintptr_t>(lists[a][0]) < reinterpret_cast<uintptr_t>(lists[b][0]); });
+  for (size_t k = 0; k < used; ++k) {
+    const size_t list = order[k];
     const int* dtypes = list == 0 ? call.param_dtypes : list == 1 ? call.grad_dtypes : nullptr;
-    Span* added = spans + list * count;
+    Span* added = spans + k * count;
+    bool rising = true;
+    uintptr_t last = 0;
     for (size_t i = 0; i < count; ++i) {
       const uintptr_t begin = reinterpret_cast<uintptr_t>(lists[list][i]);
       added[i] = {begin, begin + (dtypes && dtypes[i] != BB200_F32 ? 2 : 4) * call.numels[i]};
+      rising &= begin >= last;
+      last = begin;
     }
-    append(list * count, count);
+    append(k * count, count, rising);
   }
   const uintptr_t schedule = reinterpret_cast<uintptr_t>(call.schedule);
   spans[all - 1] = {schedule, schedule + 3 * sizeof(float)};
-  append(all - 1, 1);
+  append(all - 1, 1, true);
   size_t k = 1;
   while (k < all && spans[k - 1].end <= spans[k].begin) ++k;
   const uintptr_t first = spans[k - 1].begin, second = k < all ? spans[k].begin : 0;
