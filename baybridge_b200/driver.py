@@ -248,7 +248,48 @@ def default_cache_dir() -> Path:
     return Path(configured).expanduser() if configured else Path.home() / ".cache" / "baybridge"
 
 
-def _bind_user_arguments(definition, backend_launcher: Callable[..., Any], bindings: list[dict[str, Any]]):
+@dataclass(frozen=True)
+class _Constant:
+    """A sample argument, or a part of one, that is no argument of the IR: tracing took it as it was (``None``, a string)."""
+
+    value: Any
+
+
+def _form_of(value: Any) -> Any:
+    """What ``_proxy_for`` made of a sample: ``None`` for an IR argument, a ``_Constant``, or a dict of the same for the parts
+    of a container that are not arguments themselves."""
+    if infer_runtime_spec(value)[0] != "python_object":
+        return None
+    if isinstance(value, (list, tuple, TensorGroup)):
+        value = dict(enumerate(value))
+    if isinstance(value, dict):
+        return {key: form for key, form in ((key, _form_of(item)) for key, item in value.items()) if form is not None}
+    return _Constant(value)
+
+
+def _holds_arguments(value: Any) -> bool:
+    """Whether tracing would make an IR argument of ``value`` or of a part of it."""
+    if infer_runtime_spec(value)[0] != "python_object":
+        return True
+    if isinstance(value, dict):
+        value = list(value.values())
+    return isinstance(value, (list, tuple, TensorGroup)) and any(_holds_arguments(item) for item in value)
+
+
+def _check_form(name: str, value: Any, form: Any) -> None:
+    """Refuse a call's argument where compiling saw a constant: the launch would leave it out without a word."""
+    if isinstance(form, dict):
+        for key, part in form.items():
+            if isinstance(value, dict) and key in value or isinstance(value, (list, tuple, TensorGroup)) and isinstance(key, int) and key < len(value):
+                _check_form(f"{name}[{key!r}]", value[key], part)
+            elif isinstance(key, str) and hasattr(value, key):
+                _check_form(f"{name}.{key}", getattr(value, key), part)
+    elif isinstance(form, _Constant) and value is not form.value and _holds_arguments(value):
+        if not (type(value) is type(form.value) and isinstance(value, (bool, int, float)) and value == form.value):
+            raise TypeError(f"'{name}' is not an operand of this artifact: it was {form.value!r} when the kernel was compiled; compile it with one")
+
+
+def _bind_user_arguments(definition, backend_launcher: Callable[..., Any], bindings: list[dict[str, Any]], samples: tuple[Any, ...]):
     """User-signature call → IR-argument-order call (leaf extraction by recorded path), forwarding ``stream=``."""
     signature = inspect.signature(definition.fn)
 
@@ -268,6 +309,13 @@ def _bind_user_arguments(definition, backend_launcher: Callable[..., Any], bindi
     direct = (len(positional) == len(parameters) and "stream" not in signature.parameters
               and all(not binding["path"] and binding["parameter"] in positional for binding in bindings))
     order = [positional.index(binding["parameter"]) for binding in bindings] if direct else []
+    # what compiling took as constants; a parameter without any binding is compared in the short cuts as well (``unbound``)
+    supplied, bound_names = signature.bind_partial(*samples).arguments, {binding["parameter"] for binding in bindings}
+    given = {p.name: supplied.get(p.name, p.default) for p in parameters if p.name != "stream"}  # a stream is the launch's own
+    forms = {name: _form_of(value) if name in supplied else _Constant(value) for name, value in given.items()
+             if not any(binding["parameter"] == name and not binding["path"] for binding in bindings)}
+    forms = {name: form for name, form in forms.items() if form}
+    unbound = [(index, given[name]) for index, name in enumerate(positional) if name in given and name not in bound_names]
     # a backend launcher may offer two short cuts, which return False where the ordinary path has to look closer (and find
     # the error): ``quick(leaves, stream)``, and ``grouped(values, stream)`` for lists of leaves given as one tensor
     # group each (``values``: the argument of every parameter by the position of its first leaf)
@@ -281,12 +329,16 @@ def _bind_user_arguments(definition, backend_launcher: Callable[..., Any], bindi
     def quick(args: tuple[Any, ...], stream: Any) -> bool:
         if len(args) != len(positional):
             return False
+        for index, constant in unbound:
+            if args[index] is not constant:
+                return False
         if quick_leaves is not None:
             return quick_leaves(args if every else [args[index] for index in order], stream)
         return grouped({leaf: args[place] for place, leaf in spans}, stream)
 
     def launcher(*args: Any, **kwargs: Any) -> Any:
-        if direct and len(args) == len(positional) and (not kwargs or (len(kwargs) == 1 and "stream" in kwargs)):
+        if (direct and len(args) == len(positional) and (not kwargs or (len(kwargs) == 1 and "stream" in kwargs))
+                and all(args[index] is constant for index, constant in unbound)):
             stream = kwargs.get("stream") if kwargs else None
             leaves = [args[index] for index in order]
             for leaf in leaves:
@@ -300,6 +352,9 @@ def _bind_user_arguments(definition, backend_launcher: Callable[..., Any], bindi
         bound = signature.bind_partial(*args, **kwargs).arguments
         if stream is None and "stream" in bound:
             stream = bound["stream"]
+        for name, form in forms.items():
+            if name in bound:
+                _check_form(name, bound[name], form)
         leaves = [
             normalize_runtime_argument(pluck(bound[binding["parameter"]], binding["path"]), stream=stream)
             for binding in bindings
@@ -349,7 +404,7 @@ def _compile(kernel: Any, *sample_args: Any, target=None, backend: Any = None,
             launcher = backend_object.build_launcher(ir, target, lowered, lowered_path)
             bindings = ir.metadata.get("trace_bindings")
             if isinstance(bindings, list) and bindings:
-                launcher = _bind_user_arguments(definition, launcher, bindings)
+                launcher = _bind_user_arguments(definition, launcher, bindings, samples)
     return CompiledKernel(
         ir=ir, target=target, backend_name=backend_name, cache_key=key, artifact_path=manifest_path,
         lowered_path=lowered_path, lowered_module=lowered, debug_bundle_dir=bundle, from_cache=from_cache,

@@ -1,0 +1,109 @@
+"""Calls of a compiled artifact that differ from what it was compiled for, without a GPU: nothing is left out silently."""
+from __future__ import annotations
+
+import pytest
+from test_host_surface import FakeCudaTensor
+
+import baybridge_b200 as cute
+from baybridge_b200.backend import native
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """Entry points that only record their arguments."""
+    seen = []
+    monkeypatch.setattr(native, "entry_point", lambda name: lambda *arguments: seen.append((name, arguments)) or 0)
+    monkeypatch.setattr(native, "call", lambda *arguments: None)
+    monkeypatch.setattr(native, "take_device_status", lambda stream: 0)
+    monkeypatch.setattr(native, "require_device", lambda: None)
+    monkeypatch.setattr("baybridge_b200.backend.b200._bind_device", lambda device: None)
+    return seen
+
+
+class Tensors:
+    """Distinct stand-ins for device tensors, as exporters or as handles."""
+
+    def __init__(self, handles: bool):
+        self.place, self.handles = iter(range(1 << 20, 1 << 30, 1 << 16)), handles
+
+    def __call__(self, shape, dtype="float32"):
+        value = FakeCudaTensor(shape, dtype, next(self.place))
+        return cute.from_dlpack(value) if self.handles else value
+
+    def list(self, count, shape=(8,)):
+        return [self(shape) for _ in range(count)]
+
+    def group(self, count, shape=(8,)):
+        return cute.tensor_group(self.list(count, shape))
+
+
+def _norm(x, out, mean, rstd, weight, bias=None, residual=None, out_resid=None):
+    cute.layernorm_forward(x, out, mean, rstd, weight, bias, residual=residual, out_resid=out_resid)
+
+
+def _step(params, grads, exp_avgs, exp_avg_sqs, schedule, masters):
+    cute.adamw(params, grads, exp_avgs, exp_avg_sqs, schedule, masters=masters)
+
+
+@pytest.mark.parametrize("handles", [False, True])
+@pytest.mark.parametrize("synchronize", [False, True])
+def test_operands_left_out_at_compile_time_are_refused_at_the_call(handles, synchronize, launches, tmp_path):
+    t = Tensors(handles)
+    backend = cute.B200Backend(synchronize=synchronize)
+    required = [t((4, 16)), t((4, 16)), t((4,)), t((4,)), t((16,))]
+    given_none = cute.compile(cute.kernel(_norm), *required, None, None, None, backend=backend, cache_dir=tmp_path)
+    defaulted = cute.compile(cute.kernel(_norm), *required, backend=backend, cache_dir=tmp_path)
+    bias, residual, out_resid = t((16,)), t((4, 16)), t((4, 16))
+    for artifact in (given_none, defaulted):
+        artifact(*required, None, None, None)
+        artifact(*required, None, None, None, stream=7)
+        assert len(launches) == 2
+        with pytest.raises(TypeError, match="'bias' is not an operand"):
+            artifact(*required, bias, residual, out_resid)
+        with pytest.raises(TypeError, match="'residual' is not an operand"):
+            artifact(*required, None, residual, out_resid, stream=7)
+        with pytest.raises(TypeError, match="'out_resid' is not an operand"):
+            artifact(*required, out_resid=out_resid)
+        assert len(launches) == 2
+        launches.clear()
+    defaulted(*required)
+    whole = cute.compile(cute.kernel(_norm), *required, bias, residual, out_resid, backend=backend, cache_dir=tmp_path)
+    whole(*required, bias, residual, out_resid)
+    assert len(launches) == 2
+    with pytest.raises((TypeError, KeyError)):  # the opposite mistake
+        whole(*required, None, None, None)
+    assert len(launches) == 2
+
+
+@pytest.mark.parametrize("synchronize", [False, True])
+def test_masters_left_out_at_compile_time_are_refused_at_the_call(synchronize, launches, tmp_path):
+    t = Tensors(True)
+    lists, schedule = [t.list(2) for _ in range(4)], t((3,))
+    artifact = cute.compile(cute.kernel(_step), *lists, schedule, None, backend=cute.B200Backend(synchronize=synchronize), cache_dir=tmp_path)
+    groups = [cute.tensor_group(members) for members in lists]
+    for masters in (t.group(2), t.list(2), tuple(t.list(2)), {"a": t((8,))}):
+        for arguments in (groups, lists, [groups[0], *lists[1:]]):
+            with pytest.raises(TypeError, match="'masters' is not an operand"):
+                artifact(*arguments, schedule, masters)
+    assert not launches
+    artifact(*groups, schedule, None)
+    artifact(*lists, schedule, None)
+    artifact(*groups, schedule, [])  # holds nothing that could be left out
+    assert len(launches) == 3
+
+
+def test_constants_of_a_kernel_keep_working_and_changed_numbers_are_refused(launches, tmp_path):
+    def scaled(tokens, table, out, options, factor=2.0):
+        cute.embedding(tokens, table, out, scale=factor if options["twice"] is None else 1.0)
+
+    t = Tensors(True)
+    arguments = t((4,), "int32"), t((9, 16)), t((4, 16))
+    artifact = cute.compile(cute.kernel(scaled), *arguments, {"twice": None, "name": "a"}, backend=cute.B200Backend(synchronize=False), cache_dir=tmp_path)
+    artifact(*arguments, {"twice": None, "name": "b"})
+    artifact(*arguments, {"twice": None, "name": "a"}, 2.0)
+    assert len(launches) == 2
+    with pytest.raises(TypeError, match=r"'options\['twice'\]' is not an operand"):
+        artifact(*arguments, {"twice": t((1,)), "name": "a"})
+    with pytest.raises(TypeError, match="'factor' is not an operand of this artifact: it was 2.0"):
+        artifact(*arguments, {"twice": None, "name": "a"}, 3.0)
+    assert len(launches) == 2
