@@ -255,16 +255,24 @@ class _Constant:
     value: Any
 
 
+@dataclass(frozen=True)
+class _Container:
+    """A sample list, tuple, tensor group or dict: its keys, and the forms of the members that are not arguments themselves."""
+
+    keys: frozenset
+    by_name: bool
+    parts: tuple[tuple[Any, Any], ...]
+
+
 def _form_of(value: Any) -> Any:
-    """What ``_proxy_for`` made of a sample: ``None`` for an IR argument, a ``_Constant``, or a dict of the same for the parts
-    of a container that are not arguments themselves."""
+    """What ``_proxy_for`` made of a sample: ``None`` for an IR argument, a ``_Constant`` or a ``_Container``."""
     if infer_runtime_spec(value)[0] != "python_object":
         return None
-    if isinstance(value, (list, tuple, TensorGroup)):
-        value = dict(enumerate(value))
-    if isinstance(value, dict):
-        return {key: form for key, form in ((key, _form_of(item)) for key, item in value.items()) if form is not None}
-    return _Constant(value)
+    items = value.items() if isinstance(value, dict) else enumerate(value) if isinstance(value, (list, tuple, TensorGroup)) else None
+    if items is None:
+        return _Constant(value)
+    parts = [(key, _form_of(item)) for key, item in items]
+    return _Container(frozenset(key for key, _ in parts), isinstance(value, dict), tuple(part for part in parts if part[1] is not None))
 
 
 def _holds_arguments(value: Any) -> bool:
@@ -276,14 +284,28 @@ def _holds_arguments(value: Any) -> bool:
     return isinstance(value, (list, tuple, TensorGroup)) and any(_holds_arguments(item) for item in value)
 
 
+def _member(value: Any, step: Any) -> Any:
+    if not isinstance(value, dict) and isinstance(step, str) and hasattr(value, step):
+        return getattr(value, step)
+    return value[step]
+
+
 def _check_form(name: str, value: Any, form: Any) -> None:
-    """Refuse a call's argument where compiling saw a constant: the launch would leave it out without a word."""
-    if isinstance(form, dict):
-        for key, part in form.items():
-            if isinstance(value, dict) and key in value or isinstance(value, (list, tuple, TensorGroup)) and isinstance(key, int) and key < len(value):
-                _check_form(f"{name}[{key!r}]", value[key], part)
-            elif isinstance(key, str) and hasattr(value, key):
-                _check_form(f"{name}.{key}", getattr(value, key), part)
+    """Refuse an argument with more or fewer parts than compiling saw, or with an operand where it saw a constant: the launch
+    would leave out what it was not compiled for without a word."""
+    if isinstance(form, _Container):
+        if form.by_name:  # an object may stand in for a dict, by its attributes
+            unknown = [key for key in value if key not in form.keys and _holds_arguments(value[key])] if isinstance(value, dict) else []
+            if unknown:
+                raise TypeError(f"'{name}' holds {unknown[0]!r}, which was not there when the kernel was compiled; compile it with that")
+        elif hasattr(value, "__len__") and len(value) != len(form.keys):
+            raise TypeError(f"'{name}' has {len(value)} members, but the kernel was compiled for {len(form.keys)}")
+        for key, part in form.parts:
+            try:
+                member = _member(value, key)
+            except (KeyError, IndexError, TypeError):
+                continue  # nothing there that could be left out
+            _check_form(f"{name}[{key!r}]", member, part)
     elif isinstance(form, _Constant) and value is not form.value and _holds_arguments(value):
         if not (type(value) is type(form.value) and isinstance(value, (bool, int, float)) and value == form.value):
             raise TypeError(f"'{name}' is not an operand of this artifact: it was {form.value!r} when the kernel was compiled; compile it with one")
@@ -295,12 +317,7 @@ def _bind_user_arguments(definition, backend_launcher: Callable[..., Any], bindi
 
     def pluck(value: Any, path: list[Any]) -> Any:
         for step in path:
-            if isinstance(value, dict):
-                value = value[step]
-            elif isinstance(step, str) and hasattr(value, step):
-                value = getattr(value, step)
-            else:
-                value = value[step]
+            value = _member(value, step)
         return value
 
     parameters = list(signature.parameters.values())
@@ -314,7 +331,7 @@ def _bind_user_arguments(definition, backend_launcher: Callable[..., Any], bindi
     given = {p.name: supplied.get(p.name, p.default) for p in parameters if p.name != "stream"}  # a stream is the launch's own
     forms = {name: _form_of(value) if name in supplied else _Constant(value) for name, value in given.items()
              if not any(binding["parameter"] == name and not binding["path"] for binding in bindings)}
-    forms = {name: form for name, form in forms.items() if form}
+    forms = {name: form for name, form in forms.items() if form is not None}
     unbound = [(index, given[name]) for index, name in enumerate(positional) if name in given and name not in bound_names]
     # a backend launcher may offer two short cuts, which return False where the ordinary path has to look closer (and find
     # the error): ``quick(leaves, stream)``, and ``grouped(values, stream)`` for lists of leaves given as one tensor

@@ -107,3 +107,44 @@ def test_constants_of_a_kernel_keep_working_and_changed_numbers_are_refused(laun
     with pytest.raises(TypeError, match="'factor' is not an operand of this artifact: it was 2.0"):
         artifact(*arguments, {"twice": None, "name": "a"}, 3.0)
     assert len(launches) == 2
+
+
+@pytest.mark.parametrize("synchronize", [False, True])
+@pytest.mark.parametrize("count", [1, 3])
+def test_lists_of_another_length_are_refused(count, synchronize, launches, tmp_path):
+    t = Tensors(True)
+    schedule = t((3,))
+    artifact = cute.compile(cute.kernel(_step), *[t.list(2) for _ in range(4)], schedule, t.list(2),
+                            backend=cute.B200Backend(synchronize=synchronize), cache_dir=tmp_path)
+    lists, groups = (lambda n: [t.list(n) for _ in range(4)]), (lambda n: [t.group(n) for _ in range(4)])
+    artifact(*lists(2), schedule, t.list(2))
+    artifact(*groups(2), schedule, t.group(2))
+    artifact(t.group(2), *lists(2)[1:], schedule, tuple(t.list(2)))
+    assert len(launches) == 3
+    for arguments in (lists(count), groups(count), [t.group(count), *lists(count)[1:]], [t.list(2), *lists(count)[1:]], [*lists(2)[1:], t.list(count)]):
+        for masters in (t.list(2), t.group(2), t.list(count)):
+            with pytest.raises((TypeError, IndexError)):
+                artifact(*arguments, schedule, masters)
+    with pytest.raises(TypeError, match=f"'masters' has {count} members, but the kernel was compiled for 2"):
+        artifact(*lists(2), schedule, t.list(count))
+    assert len(launches) == 3
+
+
+def test_parts_of_a_dict_that_were_not_there_at_compile_time_are_refused(launches, tmp_path):
+    def lookup(operands):
+        cute.embedding(operands["tokens"], operands["table"], operands["out"])
+
+    t = Tensors(False)
+    operands = {"tokens": t((4,), "int32"), "table": t((9, 16)), "out": t((4, 16))}
+    artifact = cute.compile(cute.kernel(lookup), operands, backend=cute.B200Backend(synchronize=False), cache_dir=tmp_path)
+    artifact(operands)
+    artifact({**operands, "note": "not an operand"})
+
+    class Record:
+        tokens, table, out, more = (*operands.values(), t((1,)))
+
+    artifact(Record)  # an object with these attributes, and others of its own
+    assert len(launches) == 3
+    with pytest.raises(TypeError, match="'operands' holds 'more'"):
+        artifact({**operands, "more": t((1,))})
+    assert len(launches) == 3
