@@ -616,17 +616,18 @@ class B200Backend:
     def _adamw_grouped(self, ir, plan: AdamWPlan, state):
         """The step on whole tensor groups: ``grouped({position of the first leaf: value}, stream)`` launches and returns
         True when every list of the plan arrives as one ``TensorGroup``, and returns False otherwise (the caller then
-        passes the leaves one by one)."""
+        passes the leaves one by one), as it does for a kernel that steps only some members of its lists."""
         step, count = self._adamw_call(plan), len(plan.params)
         roles = [plan.params, plan.grads, plan.exp_avgs, plan.exp_avg_sqs] + ([plan.masters] if plan.masters else [])
-        contiguous = all(role == tuple(range(role[0], role[0] + count)) for role in roles)
+        whole = (all(role == tuple(range(role[0], role[0] + count)) for role in roles)
+                 and len(ir.arguments) == count * len(roles) + 1)  # no argument that the step does not take
         expected = [group_signature((ir.arguments[p].spec.dtype, ir.arguments[p].spec.shape) for p in role) for role in roles]
         names = ("params", "grads", "exp_avgs", "exp_avg_sqs", "masters")
         firsts, schedule_signature = [role[0] for role in roles], ("f32", (3,), DLPACK_CUDA, True)
 
         def grouped(values: dict[int, Any], stream: Any) -> bool:
             schedule = values.get(plan.schedule)
-            if not contiguous or type(schedule) is not TensorHandle or schedule.signature != schedule_signature or len(values) != len(roles) + 1:
+            if not whole or type(schedule) is not TensorHandle or schedule.signature != schedule_signature or len(values) != len(roles) + 1:
                 return False
             groups = [values.get(first) for first in firsts]
             for group in groups:

@@ -148,3 +148,17 @@ def test_parts_of_a_dict_that_were_not_there_at_compile_time_are_refused(launche
     with pytest.raises(TypeError, match="'operands' holds 'more'"):
         artifact({**operands, "more": t((1,))})
     assert len(launches) == 3
+
+
+def test_a_kernel_that_steps_some_members_of_its_lists_takes_groups_as_well(launches, tmp_path):
+    def step(params, grads, exp_avgs, exp_avg_sqs, schedule):
+        cute.adamw(params[:2], grads[:2], exp_avgs[:2], exp_avg_sqs[:2], schedule)
+
+    t = Tensors(True)
+    lists, schedule = [t.list(3) for _ in range(4)], t((3,))
+    artifact = cute.compile(cute.kernel(step), *lists, schedule, backend=cute.B200Backend(synchronize=False), cache_dir=tmp_path)
+    artifact(*lists, schedule)
+    artifact(*[cute.tensor_group(members) for members in lists], schedule)
+    for _, arguments in launches:
+        assert arguments[0] == 2 and [list(array) for array in arguments[5:9]] == [[m.data_ptr() for m in members[:2]] for members in lists]
+    assert len(launches) == 2
