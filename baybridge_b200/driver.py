@@ -451,10 +451,23 @@ compile = _CompileDispatcher()
 _EAGER: dict[tuple, CompiledKernel] = {}
 
 
+def _eager_signature(value: Any) -> Any:
+    """What compiling sees of an argument: dtype and shape of what becomes an argument of the IR, container by container, and
+    the names and absences that it takes as constants."""
+    spec = infer_runtime_spec(value)
+    if spec[0] != "python_object":
+        return spec
+    if isinstance(value, (list, tuple, TensorGroup)):
+        return ("list" if isinstance(value, list) else "tuple", tuple(_eager_signature(item) for item in value))
+    if isinstance(value, dict):
+        return "dict", tuple((key, _eager_signature(item)) for key, item in value.items())
+    return spec + (value,) if value is None or isinstance(value, (str, bytes)) else spec
+
+
 def run_on_device(definition, args: tuple[Any, ...], kwargs: dict[str, Any], stream: Any | None = None) -> None:
     """``kernel(...).launch(...)`` / ``jit_fn(...)`` outside a trace: compile for b200 once per signature, then launch."""
-    signature = tuple(infer_runtime_spec(value) for value in args) + tuple(
-        (name, infer_runtime_spec(value)) for name, value in sorted(kwargs.items())
+    signature = tuple(_eager_signature(value) for value in args) + tuple(
+        (name, _eager_signature(value)) for name, value in sorted(kwargs.items())
     )
     key = (definition.fn, definition.kind, definition.launch, signature)
     artifact = _EAGER.get(key)

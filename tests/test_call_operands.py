@@ -162,3 +162,28 @@ def test_a_kernel_that_steps_some_members_of_its_lists_takes_groups_as_well(laun
     for _, arguments in launches:
         assert arguments[0] == 2 and [list(array) for array in arguments[5:9]] == [[m.data_ptr() for m in members[:2]] for members in lists]
     assert len(launches) == 2
+
+
+def test_eager_launches_compile_again_for_other_lists(launches, tmp_path, monkeypatch):
+    monkeypatch.setenv("BAYBRIDGE_CACHE_DIR", str(tmp_path))
+
+    @cute.kernel
+    def step(params, grads, exp_avgs, exp_avg_sqs, schedule, mode=None):
+        cute.adamw(params, grads, exp_avgs, exp_avg_sqs, schedule, weight_decay=0.5 if mode == "decay" else 0.0)
+
+    t = Tensors(True)
+    schedule = t((3,))
+
+    def launch(lists, *mode):
+        step(*lists, schedule, *mode).launch(grid=(1, 1, 1), block=(1, 1, 1))
+        name, arguments = launches[-1]
+        return arguments[0], list(arguments[1]), list(arguments[5]), list(arguments[4])
+
+    for count, shape in ((2, (8,)), (3, (8,)), (2, (5,)), (2, (8,)), (1, (2, 2))):
+        lists = [t.list(count, shape) for _ in range(4)]
+        numel = shape[0] * (shape[1] if len(shape) > 1 else 1)
+        expected = count, [numel] * count, [member.data_ptr() for member in lists[0]], [0.0] * count
+        assert launch(lists) == expected
+        assert launch([cute.tensor_group(members) for members in lists]) == expected
+        assert launch(lists, "decay") == expected[:3] + ([0.5] * count,)
+        assert launch(lists, "none") == expected
