@@ -471,9 +471,9 @@ def _embedding_shapes(ir, tokens_spec, table_spec, rows_spec, what: str) -> tupl
     if table_spec.dtype not in FLOAT_DTYPES or rows_spec.dtype not in FLOAT_DTYPES:
         raise _unsupported(f"{what} requires f32/bf16/f16 tensors (got {table_spec.dtype}, {rows_spec.dtype})")
     vocabulary, hidden = table_spec.shape
-    for extent in (tokens_spec.numel, vocabulary, hidden):
-        if extent >= 2**31 - 1:
-            raise _unsupported(f"{what} extents must be below 2^31 - 1 (got {extent})")
+    if max(tokens_spec.numel, vocabulary) >= 2**31 - 1 or hidden > 2**30:
+        raise _unsupported(f"{what} takes fewer than 2^31 - 1 tokens and rows and at most 2^30 columns "
+                           f"(got {tokens_spec.numel}, {vocabulary}, {hidden})")
     return tokens_spec.numel, vocabulary, hidden
 
 

@@ -916,8 +916,9 @@ int check_extents(const char* what, size_t count, size_t vocabulary, size_t hidd
   if (token_dtype != BB200_I32 && token_dtype != BB200_I64)
     return fail(BB200_E_INVALID_ARGUMENT, "%s: token dtype %d is not i32/i64", what, (int)token_dtype);
   if (count == 0 || vocabulary == 0 || hidden == 0) return fail(BB200_E_INVALID_ARGUMENT, "%s: count, vocabulary and hidden must be > 0", what);
-  if (count >= 0x7fffffffu || vocabulary >= 0x7fffffffu || hidden >= 0x7fffffffu)
-    return fail(BB200_E_UNSUPPORTED_SHAPE, "%s: extents must be below 2^31 - 1", what);
+  // columns are counted in an int that runs past the row by up to a grid's stride, 65535 * 256 steps
+  if (count >= 0x7fffffffu || vocabulary >= 0x7fffffffu || hidden > (1u << 30))
+    return fail(BB200_E_UNSUPPORTED_SHAPE, "%s: count and vocabulary must be below 2^31 - 1 and hidden at most 2^30", what);
   return BB200_OK;
 }
 

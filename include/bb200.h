@@ -313,7 +313,8 @@ int bb200_attention_fwd_gather(const void* q, const void* k, const void* v, void
 /* out[t, :] = scale * table[tokens[t], :] for t < count; tokens i32 / i64, table [vocabulary, hidden], out [count, hidden]
  * row-major, each bf16 / f16 / f32; computed in f32 and rounded once.  A token outside [0, vocabulary) gets a row of zeros
  * and sets the device status word to BB200_TOKEN_OUT_OF_RANGE.  16-byte vectors where both row tensors are 16-byte
- * aligned and hidden is a multiple of 8 (4 if both are f32), single elements otherwise.  No upstream counterpart. */
+ * aligned and hidden is a multiple of 8 (4 if both are f32), single elements otherwise.  count and vocabulary below 2^31 - 1,
+ * hidden at most 2^30, here and below.  No upstream counterpart. */
 int bb200_embedding(bb200_dtype table_dtype, bb200_dtype out_dtype, bb200_dtype token_dtype, const void* tokens, const void* table,
                     void* out, size_t count, size_t vocabulary, size_t hidden, float scale, void* stream);
 
