@@ -64,6 +64,12 @@ template <> struct Sum<1> {
   __device__ __forceinline__ Pack<float, 1> values() const { return {{value}}; }
 };
 
+// A token outside the table is recorded only where nothing else is: the code of a wait that gave up, which means that some
+// output is incomplete, stays.
+__device__ __forceinline__ void record_bad_token(int* status_word) {
+  if (status_word) atomicCAS(status_word, 0, BB200_TOKEN_OUT_OF_RANGE);
+}
+
 // ---- lookup -------------------------------------------------------------------------------------------------------
 // `1 << lane_bits` neighbouring threads share a row; each has four vectors of it on their way at once.  Up to 64 threads a
 // row: 65536 rows of 4096 bf16 114 us, 124 us with two vectors a thread; f32 to bf16 156 us, 160 us with 256 threads a row.
@@ -90,7 +96,7 @@ lookup_rows(const Id* __restrict__ tokens, const T* __restrict__ table, O* __res
   if (row >= count) return;
   const long long token = (long long)tokens[row];
   const bool inside = token >= 0 && (unsigned long long)token < vocabulary;
-  if (!inside && lane == 0 && blockIdx.y == 0 && status_word) atomicExch(status_word, BB200_TOKEN_OUT_OF_RANGE);
+  if (!inside && lane == 0 && blockIdx.y == 0) record_bad_token(status_word);
   const T* __restrict__ source = table + (inside ? (size_t)token : 0) * ((size_t)steps * VEC);
   O* __restrict__ target = out + row * ((size_t)steps * VEC);
   for (int step = blockIdx.y * kUnroll * lanes + lane; step < steps; step += gridDim.y * kUnroll * lanes) {
@@ -141,7 +147,7 @@ constexpr int kCounterWords = kBins / 2 + 1;
 template <typename Id> __device__ __forceinline__ uint32_t key_of(Id raw, uint32_t vocabulary, long long padding, int* status_word) {
   const long long token = (long long)raw;
   if (token < 0 || token >= (long long)vocabulary) {
-    if (status_word) atomicExch(status_word, BB200_TOKEN_OUT_OF_RANGE);
+    record_bad_token(status_word);
     return vocabulary;
   }
   return token == padding ? vocabulary : (uint32_t)token;

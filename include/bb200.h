@@ -307,7 +307,7 @@ int bb200_attention_fwd_gather(const void* q, const void* k, const void* v, void
 
 /* ---- a training step's operators (upstream has none of them) ------------------------------------------------------ */
 
-/* Status-word code of a lookup that met a token outside its table. */
+/* Status-word code of a lookup that met a token outside its table.  It does not replace another code that waits to be read. */
 #define BB200_TOKEN_OUT_OF_RANGE 311
 
 /* out[t, :] = scale * table[tokens[t], :] for t < count; tokens i32 / i64, table [vocabulary, hidden], out [count, hidden]
