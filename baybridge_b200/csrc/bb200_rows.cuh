@@ -206,8 +206,8 @@ template <int STAGE_BYTES, int MOST_BYTES> constexpr int stages_for() {
 }
 
 // Rows of whole 16-byte vectors, 16-byte aligned.  Thread `lane` of a group owns the vectors lane, lane + LANES, ...; it
-// copies and reads them itself, so it waits for nothing but its own copies.
-template <typename T, int THREADS_, int LANES_, int VPT, int TENSORS, int MOST_BYTES> struct VectorRows {
+// copies and reads them itself, so it waits for nothing but its own copies.  FULL: the rows fill all of them.
+template <typename T, int THREADS_, int LANES_, int VPT, int TENSORS, int MOST_BYTES, bool FULL = false> struct VectorRows {
   static constexpr int THREADS = THREADS_, LANES = LANES_, VEC = 16 / sizeof(T), PAIRS = VPT * VEC / 2, GROUPS = THREADS / LANES;
   static constexpr int kSlot = THREADS * VPT * 16, kStage = kSlot * TENSORS, STAGES = stages_for<kStage, MOST_BYTES>(), kBytes = kStage * STAGES;
 
@@ -282,6 +282,9 @@ template <typename T, int THREADS_, int LANES_, int VPT, int TENSORS, int MOST_B
   __device__ __forceinline__ int column(int pair, int half) const { return vector(pair / (VEC / 2)) * VEC + pair % (VEC / 2) * 2 + half; }
   // `v` with what lies past the row's end left out
   __device__ __forceinline__ F2 inside(int pair, F2 v) const { return F2{has(pair / (VEC / 2)) ? v.bits : 0ull}; }
+  // `v`, which all columns of a row share, or zero past the row's end: one question a vector
+  static constexpr bool kMasked = true;
+  __device__ __forceinline__ F2 where_inside(int pair, float v) const { return both(FULL || has(pair / (VEC / 2)) ? v : 0.0f); }
 };
 
 // Rows of any width in tensors whose first element is 16-byte aligned: the group copies the 16-byte windows that cover the
@@ -367,6 +370,9 @@ template <typename T, int THREADS_, int LANES_, int COLUMNS, int SURE, int TENSO
     split(v, low, high);
     return make_f2(has(2 * pair) ? low : 0.0f, has(2 * pair + 1) ? high : 0.0f);
   }
+  // would be a question for every column here (8191 x 1001: 3 % of the gradient's time): `v` stays as it is
+  static constexpr bool kMasked = false;
+  __device__ __forceinline__ F2 where_inside(int, float v) const { return both(v); }
 };
 
 // A vector over the columns, of the rows' type or f32: its pairs for this thread, zeros past the row's end.

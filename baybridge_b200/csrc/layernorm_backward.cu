@@ -7,6 +7,8 @@
 // output.  A persistent CTA per SM walks groups of rows (bb200_rows.cuh); a thread keeps the two column sums of its columns
 // in registers over all its rows, and a second kernel joins the CTAs' shares in a fixed order: no atomics, the same call
 // gives the same bits.
+#include <float.h>
+
 #include "bb200_rows.cuh"
 #include "layernorm_train.h"
 
@@ -71,12 +73,20 @@ norm_backward_rows(const __grid_constant__ Backward<T> p) {
       const F2 minus_mean = both(-mean);
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {
-        n[i] = (n[i] + minus_mean) * factor;
+        n[i] = (n[i] + minus_mean) * rows.where_inside(i, rstd);
         grad_weight[i] = fma2(g[i], n[i], grad_weight[i]);
         grad_bias[i] = grad_bias[i] + g[i];
         g[i] = g[i] * weight[i];
         sum_g = sum_g + g[i];
         sum_gn = fma2(g[i], n[i], sum_gn);
+      }
+      // past the row's end x and g are 0 and n, left alone, is -mean * rstd: where that overflows, 0 * n makes the sum NaN
+      if constexpr (!Rows::kMasked) {
+        if (!(fabsf(mean * rstd) <= FLT_MAX)) {
+          sum_gn = both(0.0f);
+#pragma unroll
+          for (int i = 0; i < PAIRS; ++i) sum_gn = fma2(g[i], rows.inside(i, n[i]), sum_gn);
+        }
       }
     }
     float sums[2] = {total(sum_g), total(sum_gn)};
@@ -297,15 +307,24 @@ template <typename T, typename Rows, bool RESIDUAL, bool MAY_CLUSTER> int launch
   return workspace.release("cudaFreeAsync(layernorm_backward workspace)");
 }
 
+// Rows that fill all vectors of a group have nothing past their end to ask about, which is worth kernels of their own for the
+// wide ones (65536 x 4096 bf16 261 and 267 us, 65536 x 8192 with residual equal; up to 1024 columns no difference either).
+template <typename T, int LANES, int VPT, bool RESIDUAL> int launch_vectors(const Backward<T>& p, cudaStream_t stream) {
+  constexpr int TENSORS = RESIDUAL ? 3 : 2;
+  if constexpr (LANES >= 128) {
+    if (p.hidden == LANES * VPT * 16 / (int)sizeof(T))
+      return launch_rows<T, VectorRows<T, kRowThreads, LANES, VPT, TENSORS, kMostSmem, true>, RESIDUAL, true>(p, stream);
+  }
+  return launch_rows<T, VectorRows<T, kRowThreads, LANES, VPT, TENSORS, kMostSmem>, RESIDUAL, true>(p, stream);
+}
+
 template <typename T> int backward(Backward<T> p, bool aligned, cudaStream_t stream) {
   constexpr int VEC = 16 / sizeof(T);
   const int nvec = p.hidden / VEC;
   if (aligned && p.hidden % VEC == 0) {
     // two vectors a thread (16 columns, 8 for f32): weight, both column sums and the row's two products fit the registers
-#define BB200_VECTOR_ROWS(LANES, VPT)                                                                                  \
-  if (nvec <= (LANES) * (VPT))                                                                                         \
-    return p.grad_resid ? launch_rows<T, VectorRows<T, kRowThreads, LANES, VPT, 3, kMostSmem>, true, true>(p, stream)        \
-                        : launch_rows<T, VectorRows<T, kRowThreads, LANES, VPT, 2, kMostSmem>, false, true>(p, stream)
+#define BB200_VECTOR_ROWS(LANES, VPT) \
+  if (nvec <= (LANES) * (VPT)) return p.grad_resid ? launch_vectors<T, LANES, VPT, true>(p, stream) : launch_vectors<T, LANES, VPT, false>(p, stream)
     BB200_VECTOR_ROWS(4, 2);
     BB200_VECTOR_ROWS(8, 2);
     BB200_VECTOR_ROWS(16, 2);
