@@ -216,8 +216,9 @@ class B200Backend:
                         # that returned non-zero (upstream hipcc_exec.py:181-182)
                         status = native.take_device_status(stream_handle)
                         if status == native.TOKEN_OUT_OF_RANGE:
-                            raise RuntimeError(f"launch_{ir.name} returned device status {status}: a token of this lookup, or of one before "
-                                               "that was not waited for, lies outside the table")
+                            whose = ("this lookup, or of one before that was not waited for," if plan.kind in ("embedding", "embedding_backward")
+                                     else "a lookup before this launch, which was not waited for,")
+                            raise RuntimeError(f"launch_{ir.name} returned device status {status}: a token of {whose} lies outside the table")
                         if status:
                             raise RuntimeError(f"launch_{ir.name} returned device status {status}: a bounded device-side wait "
                                                f"gave up ({native.ERROR_NAMES[-6]}); the output is incomplete")

@@ -187,3 +187,17 @@ def test_eager_launches_compile_again_for_other_lists(launches, tmp_path, monkey
         assert launch([cute.tensor_group(members) for members in lists]) == expected
         assert launch(lists, "decay") == expected[:3] + ([0.5] * count,)
         assert launch(lists, "none") == expected
+
+
+def test_a_bad_token_found_by_a_later_launch_is_not_called_that_launchs_own(launches, tmp_path, zoo, monkeypatch):
+    t = Tensors(True)
+    a, b, c = t((256, 256), "bfloat16"), t((256, 256), "bfloat16"), t((256, 256), "bfloat16")
+    tokens, table, out = t((4,), "int32"), t((9, 16)), t((4, 16))
+    product = cute.compile(zoo.gemm_abt, a, b, c, backend="b200", cache_dir=tmp_path)
+    lookup = cute.compile(zoo.make_embedding(), tokens, table, out, backend="b200", cache_dir=tmp_path)
+    monkeypatch.setattr(native, "call_resolved", lambda *arguments: None)
+    monkeypatch.setattr(native, "take_device_status", lambda stream: native.TOKEN_OUT_OF_RANGE)
+    with pytest.raises(RuntimeError, match="device status 311: a token of a lookup before this launch, which was not waited for, lies outside the table"):
+        product(a, b, c)
+    with pytest.raises(RuntimeError, match="device status 311: a token of this lookup, or of one before that was not waited for, lies outside the table"):
+        lookup(tokens, table, out)
