@@ -193,7 +193,7 @@ class B200Backend:
                 raise TypeError(f"{ir.name} expects {len(arguments)} arguments, got {len(args)}")
             native.require_device()
             synchronize = self.synchronize and not native.recording()  # a recording stream must not be synchronised
-            if all_tensors and quick(args, stream):
+            if all_tensors and not synchronize and quick(args, stream):
                 return
             staged: list[tuple[RuntimeTensor, _StagedSlot, Any]] = []
             stream_handle = native.stream_handle(stream)
@@ -246,7 +246,7 @@ class B200Backend:
                     native.library().bb200_module_unload(module)
                 holder.get("functions", {}).clear()
 
-        if all_tensors:
+        if all_tensors and not self.synchronize:  # a synchronising launcher would only be asked in vain
             launcher.quick = quick  # type: ignore[attr-defined]
         if isinstance(plan, AdamWPlan):
             launcher.grouped = self._adamw_grouped(ir, plan, state)  # type: ignore[attr-defined]

@@ -217,9 +217,15 @@ class CompiledKernel:
             )
         stream = kwargs.get("stream") if kwargs else None
         # the hot call: device tensor handles (or groups of them) as they were compiled for need no normalisation
-        quick = getattr(self.runtime_callable, "quick", None)
-        if quick is not None and (not kwargs or (len(kwargs) == 1 and "stream" in kwargs)) and quick(args, stream):
-            return None
+        if not kwargs or (len(kwargs) == 1 and "stream" in kwargs):
+            quick = getattr(self.runtime_callable, "quick", None)
+            if quick is not None and quick(args, stream):
+                return None
+            for arg in args:
+                if type(arg) is not TensorHandle:
+                    break
+            else:
+                return self.runtime_callable(*args, **kwargs)
         args = tuple(normalize_runtime_argument(arg, stream=stream) for arg in args)
         kwargs = {
             name: value if name == "stream" else normalize_runtime_argument(value, stream=stream)
@@ -355,7 +361,7 @@ def _bind_user_arguments(definition, backend_launcher: Callable[..., Any], bindi
 
     def launcher(*args: Any, **kwargs: Any) -> Any:
         if (direct and len(args) == len(positional) and (not kwargs or (len(kwargs) == 1 and "stream" in kwargs))
-                and all(args[index] is constant for index, constant in unbound)):
+                and (not unbound or all(args[index] is constant for index, constant in unbound))):
             stream = kwargs.get("stream") if kwargs else None
             leaves = [args[index] for index in order]
             for leaf in leaves:

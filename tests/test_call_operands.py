@@ -201,3 +201,18 @@ def test_a_bad_token_found_by_a_later_launch_is_not_called_that_launchs_own(laun
         product(a, b, c)
     with pytest.raises(RuntimeError, match="device status 311: a token of this lookup, or of one before that was not waited for, lies outside the table"):
         lookup(tokens, table, out)
+
+
+@pytest.mark.parametrize("synchronize", [False, True])
+def test_calls_on_handles_are_not_looked_over_twice(synchronize, launches, tmp_path, zoo, monkeypatch):
+    """Device tensor handles need no normalisation, whether the launcher synchronises or not, and a launcher that waits for its
+    kernel, which the short path cannot do, is not asked for the short path."""
+    t = Tensors(True)
+    handles = t((4,), "int32"), t((9, 16)), t((4, 16))
+    artifact = cute.compile(zoo.make_embedding(), *handles, backend=cute.B200Backend(synchronize=synchronize), cache_dir=tmp_path)
+    normalised = []
+    monkeypatch.setattr("baybridge_b200.driver.normalize_runtime_argument", lambda value, stream=None: normalised.append(value) or value)
+    artifact(*handles)
+    artifact(*handles, stream=3)
+    assert len(launches) == 2 and not normalised
+    assert hasattr(artifact.runtime_callable, "quick") is not synchronize
