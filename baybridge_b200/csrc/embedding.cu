@@ -756,29 +756,38 @@ int launch_cluster_sort(const GradientCall& call, unsigned ctas, int passes, int
   return check_launch("embedding_backward sort launch");
 }
 
-// Sorts the call's tokens into `list`.  `spare`: as much again, for the passes between, and `counts`, where there are more
-// than one cluster holds.
+struct ClusterShape {
+  unsigned ctas = 0;  // 0: no cluster holds the tokens
+  int rounds = 0;     // elements a thread
+};
+
+// The cluster that sorts `count` tokens: few elements a thread and many CTAs (65536 tokens: 24 us with 16 CTAs, 35 us with eight of
+// twice the elements).  65536 tokens at most, half as many on a device that cannot hold clusters of 16.
+template <typename Id> ClusterShape cluster_for(uint32_t count) {
+  const auto ctas = [count](uint32_t rounds) {  // a power of two
+    unsigned n = 1;
+    while (n < 32 && n * rounds * kSortThreads < count) n *= 2;
+    return n;
+  };
+  const unsigned one = ctas(1), two = ctas(2), four = ctas(4);
+  if (one <= 8 || (one == 16 && sixteen_fit<sort_in_cluster<Id, 1>>(kSortThreads, sizeof(ClusterSort<1>)))) return {one, 1};
+  if (two <= 8 || (two == 16 && sixteen_fit<sort_in_cluster<Id, 2>>(kSortThreads, sizeof(ClusterSort<2>)))) return {two, 2};
+  if (four <= 8 || (four == 16 && sixteen_fit<sort_in_cluster<Id, 4>>(kSortThreads, sizeof(ClusterSort<4>)))) return {four, 4};
+  return {};
+}
+
+// Sorts the call's tokens into `list`, in `cluster` where there is one.  `spare`: as much again, for the passes between, and
+// `counts`, where there is none.
 template <typename Id>
-int sort_tokens(const GradientCall& call, const SortedList& list, const SortedList& spare, uint32_t* counts, uint8_t* named, size_t zero_bytes,
-                cudaStream_t stream) {
+int sort_tokens(const GradientCall& call, const ClusterShape& cluster, const SortedList& list, const SortedList& spare, uint32_t* counts,
+                uint8_t* named, size_t zero_bytes, cudaStream_t stream) {
   const uint32_t count = (uint32_t)call.count, vocabulary = (uint32_t)call.vocabulary;
   int bits = 1;  // of the keys 0 .. vocabulary
   while (((unsigned long long)call.vocabulary >> bits) != 0) ++bits;
   const int passes = (bits + kDigitBits - 1) / kDigitBits, digit_bits = (bits + passes - 1) / passes;
-  // Few elements a thread and many CTAs (65536 tokens: 24 us with 16 CTAs, 35 us with eight of twice the elements).
-  const auto ctas = [count](uint32_t each) {  // a power of two
-    unsigned n = 1;
-    while (n * each < count) n *= 2;
-    return n;
-  };
-  const unsigned one = ctas(1024), two = ctas(2048), four = ctas(4096), eight = ctas(8192);
-  if (one <= 8 || (one == 16 && sixteen_fit<sort_in_cluster<Id, 1>>(kSortThreads, sizeof(ClusterSort<1>))))
-    return launch_cluster_sort<Id, 1>(call, one, passes, digit_bits, list, named, zero_bytes, stream);
-  if (two <= 8 || (two == 16 && sixteen_fit<sort_in_cluster<Id, 2>>(kSortThreads, sizeof(ClusterSort<2>))))
-    return launch_cluster_sort<Id, 2>(call, two, passes, digit_bits, list, named, zero_bytes, stream);
-  if (four <= 8 || (four == 16 && sixteen_fit<sort_in_cluster<Id, 4>>(kSortThreads, sizeof(ClusterSort<4>))))
-    return launch_cluster_sort<Id, 4>(call, four, passes, digit_bits, list, named, zero_bytes, stream);
-  if (eight <= 8) return launch_cluster_sort<Id, 8>(call, eight, passes, digit_bits, list, named, zero_bytes, stream);
+  if (cluster.rounds == 1) return launch_cluster_sort<Id, 1>(call, cluster.ctas, passes, digit_bits, list, named, zero_bytes, stream);
+  if (cluster.rounds == 2) return launch_cluster_sort<Id, 2>(call, cluster.ctas, passes, digit_bits, list, named, zero_bytes, stream);
+  if (cluster.rounds == 4) return launch_cluster_sort<Id, 4>(call, cluster.ctas, passes, digit_bits, list, named, zero_bytes, stream);
   const Id* tokens = static_cast<const Id*>(call.tokens);
   const int tiles = (int)((call.count + kTile - 1) / kTile);
   const uint32_t mask = (1u << digit_bits) - 1;
@@ -855,7 +864,8 @@ template <typename G, typename W, int VEC, bool ADD> int gradient(const Gradient
   while (2 * s.chunk_length * groups <= (size_t)kStagedList && s.chunk_length < 512 && count * columns > (size_t)s.chunk_length * resident * 4)
     s.chunk_length *= 2;
   s.chunks = (uint32_t)((count + s.chunk_length - 1) / s.chunk_length);
-  const bool spare = count > 65536;
+  const ClusterShape cluster = wide_tokens ? cluster_for<int64_t>(s.count) : cluster_for<int32_t>(s.count);
+  const bool spare = !cluster.ctas;
   const size_t list = round_up(count * 4), crossings = round_up((2 + (size_t)s.chunks) * 4);
   const size_t counts_bytes = spare ? round_up((count + kTile - 1) / kTile * kBins * 4) : 0, partial = round_up((size_t)s.chunks * 2 * call.hidden * 4);
   const size_t named_bytes = ADD ? 0 : round_up(call.vocabulary);
@@ -889,8 +899,8 @@ template <typename G, typename W, int VEC, bool ADD> int gradient(const Gradient
     early_rows = most < all ? most : all;
   }
   const size_t zero_bytes = early_rows * call.hidden * sizeof(W);
-  if (int status = wide_tokens ? sort_tokens<int64_t>(call, sorted, other, counts, named, zero_bytes, stream)
-                               : sort_tokens<int32_t>(call, sorted, other, counts, named, zero_bytes, stream))
+  if (int status = wide_tokens ? sort_tokens<int64_t>(call, cluster, sorted, other, counts, named, zero_bytes, stream)
+                               : sort_tokens<int32_t>(call, cluster, sorted, other, counts, named, zero_bytes, stream))
     return status;
   s.fill_from = (uint32_t)early_rows;
   s.keys = sorted.keys;
