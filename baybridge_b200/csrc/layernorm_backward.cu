@@ -183,7 +183,8 @@ norm_backward_rows(const __grid_constant__ Backward<T> p) {
   }
 }
 
-// Any width and alignment: grad_x of one row per CTA, element by element, reading the row twice (the second time from L2).
+// Any width and alignment (rows of more than 8192 columns, of more than 4096 in f32 where they are no whole vectors): grad_x of one
+// row per CTA, element by element, reading the row twice (the second time from L2); 16384 x 12288 bf16 767 us, 16384 x 8192 above 156 us.
 constexpr int kElementThreads = 256;
 template <typename T> __device__ __forceinline__ float weight_at(const Backward<T>& p, int c) {
   return p.wide ? static_cast<const float*>(p.weight)[c] : Conv<float, T>::widen(static_cast<const T*>(p.weight)[c]);

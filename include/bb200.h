@@ -322,8 +322,8 @@ int bb200_embedding(bb200_dtype table_dtype, bb200_dtype out_dtype, bb200_dtype 
  * names become zero); with accumulate != 0 the sums are added to the rows that tokens name and other rows are not
  * touched.  Tokens equal to padding_token (-1: none) contribute nothing; tokens outside [0, vocabulary) neither, and they
  * set the status word as above.  Sums are f32 in an order fixed by the token positions: the same call gives the same
- * bits.  The tokens are sorted in a workspace from the library's pool, taken and given back in stream order.  No upstream
- * counterpart. */
+ * bits.  Up to 1024 tokens of few columns take one launch and no workspace; otherwise the tokens are sorted in a workspace from
+ * the library's pool, taken and given back in stream order.  No upstream counterpart. */
 int bb200_embedding_backward(bb200_dtype grad_dtype, bb200_dtype table_dtype, bb200_dtype token_dtype, const void* grad_out,
                              const void* tokens, void* grad_table, size_t count, size_t vocabulary, size_t hidden, float scale,
                              int64_t padding_token, int accumulate, void* stream);
@@ -331,7 +331,8 @@ int bb200_embedding_backward(bb200_dtype grad_dtype, bb200_dtype table_dtype, bb
 /* s = x (+ residual, stored to out_resid); out = (s - mean) * rstd * weight + bias; mean and rstd = 1 / sqrt(var + epsilon)
  * (biased variance) of every row are stored for the backward pass.  residual / out_resid are both given or both NULL,
  * bias may be NULL.  x, residual, out, out_resid: [rows, hidden] row-major, bf16 / f16 / f32; weight, bias: [hidden], of that
- * dtype or f32; hidden at most 32768 (16-bit) / 16384 (f32), any value and alignment (multiples of 16 bytes are faster).
+ * dtype or f32; hidden at most 32768 (16-bit) / 16384 (f32), any value and alignment (multiples of 16 bytes are faster, and so are
+ * rows of at most 8192 columns).
  * out_resid may be x or residual itself; no other output may share memory with another tensor.  f32 arithmetic, one
  * rounding per output.  No upstream counterpart (upstream's LayerNorm keeps no statistics: src/baybridge/frontend.py:3754-3793). */
 int bb200_layernorm_forward(bb200_dtype dtype, bb200_dtype weight_dtype, const void* x, const void* residual, const void* weight,
@@ -340,7 +341,8 @@ int bb200_layernorm_forward(bb200_dtype dtype, bb200_dtype weight_dtype, const v
 
 /* With n = (x - mean) * rstd and g = grad_out * weight: grad_x = rstd * (g - mean(g) - n * mean(g * n)) (+ grad_resid if not
  * NULL); grad_weight = sum over rows of grad_out * n; grad_bias (if not NULL) = sum over rows of grad_out.  Shapes, dtypes
- * and limits as above, grad_weight and grad_bias of the weight's dtype; no output may share memory with another tensor.
+ * and limits as above, grad_weight and grad_bias of the weight's dtype; no output may share memory with another tensor.  Rows of
+ * more than 8192 columns (f32 that are no multiple of 4: 4096) are read element by element, and more than once.
  * The column sums run in a fixed order (the same call gives the same bits) through a workspace from the library's pool,
  * taken and given back in stream order.  No upstream counterpart. */
 int bb200_layernorm_backward(bb200_dtype dtype, bb200_dtype weight_dtype, const void* grad_out, const void* x, const float* mean,
