@@ -20,6 +20,7 @@ from __future__ import annotations
 import hashlib
 import inspect
 import json
+import operator
 import os
 from dataclasses import dataclass
 from pathlib import Path
@@ -348,6 +349,7 @@ def _bind_user_arguments(definition, backend_launcher: Callable[..., Any], bindi
     spans = [(positional.index(binding["parameter"]), leaf) for leaf, binding in enumerate(bindings)
              if grouped is not None and binding["path"] in ([], [0])]
     every = order == list(range(len(positional)))
+    pick = operator.itemgetter(*order) if len(order) > 1 else lambda args: [args[index] for index in order]
 
     def quick(args: tuple[Any, ...], stream: Any) -> bool:
         if len(args) != len(positional):
@@ -356,7 +358,7 @@ def _bind_user_arguments(definition, backend_launcher: Callable[..., Any], bindi
             if args[index] is not constant:
                 return False
         if quick_leaves is not None:
-            return quick_leaves(args if every else [args[index] for index in order], stream)
+            return quick_leaves(args if every else pick(args), stream)
         return grouped({leaf: args[place] for place, leaf in spans}, stream)
 
     def launcher(*args: Any, **kwargs: Any) -> Any:
