@@ -33,6 +33,7 @@ int fail(int status, const char* fmt, ...) {
 
 int check_runtime(cudaError_t err, const char* what) {
   if (err == cudaSuccess) return BB200_OK;
+  cudaGetLastError();  // reported here: the next launch's check must not find it again
   return fail((int)err, "%s: %s (%s)", what, cudaGetErrorString(err), cudaGetErrorName(err));
 }
 

@@ -39,3 +39,24 @@ def test_a_bad_token_does_not_replace_the_code_of_a_wait_that_gave_up(gradient, 
     artifact(*arguments, stream=torch.cuda.current_stream())
     assert native.take_device_status(stream) == GIVE_UP
     assert native.take_device_status(stream) == 0
+
+
+def test_a_call_that_finds_no_memory_for_its_workspace_leaves_the_next_one_alone():
+    """The workspace's size follows from the extents alone: two rows of 2^22 f32 for each chunk of at most 512 of 2^24 tokens, 1.1
+    TB, so the call ends on the host before any launch.  What it leaves must not be taken for a failure of the next one."""
+    import torch
+    from gpu_util import void_p
+
+    from baybridge_b200 import CudaDriverError
+    from baybridge_b200.backend import native
+
+    rows, grad, table = torch.ones(4, 16, device="cuda"), torch.ones(4, 16, device="cuda"), torch.zeros(9, 16, device="cuda")
+    tokens = torch.arange(4, device="cuda", dtype=torch.int32)
+    count, hidden = 2 ** 24, 2 ** 22
+    assert count // 512 * 2 * hidden * 4 > 4 * torch.cuda.get_device_properties(0).total_memory
+    with pytest.raises(CudaDriverError, match="workspace.*cudaErrorMemoryAllocation"):
+        native.call("bb200_embedding_backward", 0, 0, 3, 1 << 50, void_p(tokens), 1 << 52, count, 1, hidden, 1.0, -1, 1, current_stream())
+    native.call("bb200_embedding", 0, 0, 3, void_p(tokens), void_p(table), void_p(rows), 4, 9, 16, 1.0, current_stream())
+    assert not rows.any()
+    native.call("bb200_embedding_backward", 0, 0, 3, void_p(grad), void_p(tokens), void_p(table), 4, 9, 16, 1.0, -1, 0, current_stream())
+    assert bool((table[:4] == 1).all()) and not table[4:].any()
