@@ -4,10 +4,10 @@
 //   gradient:  grad_table[v, :] (= or +=) scale * sum over t with token[t] = v of grad_out[t, :]
 //
 // Both are bound by HBM bytes: the lookup reads every named row and writes out once, repeats from L2 while they are still
-// there (65536 tokens: 1.3 to 1.6 times the distinct rows' bytes from DRAM); the gradient reads grad_out once and writes the table once (or reads and writes the named rows, when added).  Sums are
-// fp32 and run in an order that the token positions alone fix, so the same call gives the same bits; no floating-point
-// atomics.  Few tokens of few columns take one launch that finds the places of every token by comparing (sum_few); the
-// gradient's steps otherwise:
+// there (65536 tokens: 1.3 to 1.6 times the distinct rows' bytes from DRAM); the gradient reads grad_out once and writes the
+// table once (or reads and writes the named rows, when added).  Sums are fp32 and run in an order that the token positions
+// alone fix, so the same call gives the same bits; no floating-point atomics.  Few tokens of few columns take one launch
+// that finds the places of every token by comparing (sum_few); the gradient's steps otherwise:
 //
 //   1. a stable radix sort of (token, position) — one launch for up to 65536 tokens, held in the shared memory of a cluster
 //      of CTAs, else a histogram and a scatter launch per digit;
